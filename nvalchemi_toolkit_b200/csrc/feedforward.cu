@@ -1,0 +1,402 @@
+// SPDX-License-Identifier: Apache-2.0
+// Gated feed-forward block  y = (act(x Wg) * (x Wu)) Wd  and its backward pass, for 16-bit and float32 matrices.
+//
+// Forward: one kernel forms both projections of a tile side by side (the B tile's halves come from Wg and Wu, so one
+// instruction feeds both accumulators), applies the activation and the product in its epilogue and stores h only; a second
+// product gives y.  Backward: with g = x Wg, u = x Wu, dh = dy Wd^T
+//     dg = dh u act'(g),  du = dh act(g),  dx = dg Wg^T + du Wu^T,  dWg = x^T dg,  dWu = x^T du,  dWd = h^T dy.
+// g and u are formed again in the kernel that forms dh (three accumulators of one tile) instead of being kept: at the widths
+// of per-atom networks (K <= 1024) the extra 4 M K H operations cost less than writing and reading 2 M H values in 32 bits,
+// and 16-bit copies would add their rounding to every gradient.  What is rounded to 16 bits is what the next product reads:
+// h, dg and du, once each.
+//
+// float32 matrices run on the same tensor cores: a value is the exact sum of three bf16 values and a product the six
+// partial products down to 2^-24; the intermediate h, dg and du are stored as three planes each, so nothing is lost to
+// 16 bits.
+#include "dense16.cuh"
+
+namespace nva {
+using at::Tensor;
+namespace {
+using namespace dense;
+
+enum Act : int { kSilu = 0, kGelu = 1 };
+
+// act(g) and act'(g); EXACT: float32 results (library exponential and division), else the fast ones (1e-6 relative).
+template <bool EXACT>
+__device__ __forceinline__ void activate(int act, float g, float& a, float& da) {
+  if (act == kSilu) {
+    const float s = EXACT ? 1.f / (1.f + expf(-g)) : __fdividef(1.f, 1.f + __expf(-g));
+    a = g * s;
+    da = s * (1.f + g * (1.f - s));
+  } else {  // g * Phi(g)
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+    a = g * cdf;
+    da = cdf + g * 0.39894228040143268f * (EXACT ? expf(-0.5f * g * g) : __expf(-0.5f * g * g));
+  }
+}
+
+// Stores 32 columns of a warp's 32 rows as T, or as three bf16 planes of a float32 value.
+template <typename T>
+__device__ __forceinline__ void store32(uint4* stage, float (&v)[32], void* dst, int64_t off, int64_t ld, int64_t plane, int rows_left,
+                                        int cols_left, bool vec_ok) {
+  if constexpr (sizeof(T) == 2) {
+    uint4 o[4];
+    pack32<T>(v, o);
+    store_piece<T, 4>(stage, o, (T*)dst + off, ld, rows_left, cols_left, vec_ok);
+  } else {
+    float p1[32], p2[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float a, b, c;
+      split3(v[j], a, b, c);
+      v[j] = a; p1[j] = b; p2[j] = c;
+    }
+    uint4 o[4];
+    __nv_bfloat16* d = (__nv_bfloat16*)dst + off;
+    pack32<__nv_bfloat16>(v, o);
+    store_piece<__nv_bfloat16, 4>(stage, o, d, ld, rows_left, cols_left, vec_ok);
+    pack32<__nv_bfloat16>(p1, o);
+    store_piece<__nv_bfloat16, 4>(stage, o, d + plane, ld, rows_left, cols_left, vec_ok);
+    pack32<__nv_bfloat16>(p2, o);
+    store_piece<__nv_bfloat16, 4>(stage, o, d + 2 * plane, ld, rows_left, cols_left, vec_ok);
+  }
+}
+
+// Columns [0, BN/2) of the accumulator: g, [BN/2, BN): u, both of the same BN/2 columns of h.
+template <typename T, int BN>
+struct EpiGated {
+  static constexpr int kAcc = sizeof(T) == 4 ? 512 / BN : 1, kStride = BN;
+  struct Params { void* h; int64_t ld, plane; int act; };
+  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
+                                             uint4* stage) {
+    const int used = used_acc<kAcc>(t, at, 0);
+#pragma unroll 1
+    for (int cb = 0; cb < BN / 128; ++cb) {
+      const int c = half * (BN / 4) + cb * 32, n0 = at.n * (BN / 2) + c;
+      float g[32], u[32];
+      acc_ld32<kAcc, kStride>(tm + c, g, used);
+      acc_ld32<kAcc, kStride>(tm + BN / 2 + c, u, used);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        float a, da;
+        activate<sizeof(T) == 4>(p.act, g[j], a, da);
+        g[j] = a * u[j];
+      }
+      store32<T>(stage, g, p.h, (int64_t)row0 * p.ld + n0, p.ld, p.plane, t.M - row0, t.N - n0, true);
+    }
+  }
+};
+
+// Columns [0, 64): g, [64, 128): u, [128, 192): dh of 64 columns.
+template <typename T>
+struct EpiGatedGrad {
+  static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1, kStride = 192;
+  struct Params { void *dg, *du, *h; int64_t ld, plane; int act; };
+  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
+                                             uint4* stage) {
+    const int c = half * 32, n0 = at.n * 64 + c;
+    float g[32], u[32], d[32];
+    const int used = used_acc<kAcc>(t, at, 0);
+    acc_ld32<kAcc, kStride>(tm + c, g, used);
+    acc_ld32<kAcc, kStride>(tm + 64 + c, u, used);
+    acc_ld32<kAcc, kStride>(tm + 128 + c, d, used_acc<kAcc>(t, at, 1));
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float a, da;
+      activate<sizeof(T) == 4>(p.act, g[j], a, da);
+      g[j] = d[j] * u[j] * da;
+      d[j] *= a;
+      u[j] *= a;
+    }
+    const int64_t off = (int64_t)row0 * p.ld + n0;
+    store32<T>(stage, g, p.dg, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
+    store32<T>(stage, d, p.du, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
+    store32<T>(stage, u, p.h, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
+  }
+};
+
+// Copies a matrix into rows on 16-byte boundaries (T 16-bit), or splits float32 into three bf16 planes.  Two elements a thread.
+template <typename T, int P>
+__global__ void pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ dst,
+                            int64_t ldp, int64_t plane) {
+  const int64_t half = (cols + 1) / 2;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < rows * half; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / half, c = (i - r * half) * 2;
+    const bool two = c + 1 < cols;
+    const T* s = src + r * ld + c;
+    uint16_t* d = dst + r * ldp + c;
+    if constexpr (P == 1) {
+      const uint16_t* s16 = reinterpret_cast<const uint16_t*>(s);
+      *reinterpret_cast<uint32_t*>(d) = (uint32_t)s16[0] | (two ? (uint32_t)s16[1] << 16 : 0u);
+    } else {
+      float a[3], b[3] = {0.f, 0.f, 0.f};
+      split3((float)s[0], a[0], a[1], a[2]);
+      if (two) split3((float)s[1], b[0], b[1], b[2]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(d + k * plane) = pack2(a[k], b[k], __nv_bfloat16{});
+    }
+  }
+}
+
+// out = sum over splits of partial [splits][n], in order.
+template <typename T>
+__global__ void split_sum_kernel(const float* __restrict__ partial, int splits, int64_t stride, int64_t n, T* __restrict__ out) {
+  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+  for (int k = 0; k < splits; ++k) s += partial[k * stride + i];
+  out[i] = narrow<T>(s);
+}
+
+// A matrix as a product reads it.  `mn` says whether the axis that is not contracted is contiguous, when the contraction
+// runs over axis `k_axis` of the logical matrix.
+struct Operand {
+  Stored s;
+  Tensor keep;
+  bool rowmajor = true;
+  bool mn(int k_axis) const { return rowmajor != (k_axis == 1); }
+  int64_t extent(int axis) const { return (axis == 1) == rowmajor ? s.inner : s.outer; }
+};
+
+int planes_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? 3 : 1; }
+
+Operand operand(Tensor t, cudaStream_t st) {
+  Operand o;
+  if (t.stride(1) != 1 && t.size(1) != 1) {
+    if (t.stride(0) == 1 || t.size(0) == 1) { t = t.t(); o.rowmajor = false; }
+    else t = t.contiguous();
+  }
+  const int64_t rows = t.size(0), cols = t.size(1), ld = rows > 1 ? t.stride(0) : cols;
+  if (planes_of(t) == 1 && (rows == 1 || (ld % 8 == 0 && ld >= cols)) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) {
+    o.keep = t;
+    o.s = {t.data_ptr(), cols, rows, ld, 1, 0};
+    return o;
+  }
+  const int P = planes_of(t);
+  const int64_t ldp = (cols + 7) / 8 * 8;
+  o.keep = at::empty({P, rows, ldp}, t.options().dtype(P == 3 ? at::kBFloat16 : t.scalar_type()));
+  const int64_t work = rows * ((cols + 1) / 2);
+  const unsigned grid = (unsigned)std::min<int64_t>((work + 255) / 256, 148 * 16);
+  uint16_t* d = (uint16_t*)o.keep.data_ptr();
+  if (P == 3) pack_kernel<float, 3><<<grid, 256, 0, st>>>(t.data_ptr<float>(), ld, rows, cols, d, ldp, rows * ldp);
+  else pack_kernel<__half, 1><<<grid, 256, 0, st>>>((const __half*)t.data_ptr(), ld, rows, cols, d, ldp, 0);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  o.s = {o.keep.data_ptr(), cols, rows, ldp, P, rows * ldp};
+  return o;
+}
+
+// Intermediate [P][rows][ld] (16-bit) that epilogues write and later products read.
+Operand intermediate(int64_t rows, int64_t cols, int P, const Tensor& like, int copies = 1) {
+  Operand o;
+  const int64_t ld = (cols + 7) / 8 * 8;
+  o.keep = at::empty({copies * P, rows, ld}, like.options().dtype(P == 3 ? at::kBFloat16 : like.scalar_type()));
+  o.s = {o.keep.data_ptr(), cols, rows, ld, copies * P, rows * ld};
+  return o;
+}
+
+struct Plan {
+  Maps maps;
+  Tiles t{};
+  int n_maps = 0, P;
+  bool bf16;
+  Plan(int P_, bool bf16_) : P(P_), bf16(bf16_) {}
+  int map(const Operand& o) { put_map(maps, n_maps, o.s); return n_maps++; }
+  // a[.., k] . b[.., k]; ka / kb: the axis of each logical matrix that is contracted; b2 < 0: both halves from b.
+  // part 0: the small partial products of float32 operands (added first), 1: the large one, 2: both.
+  void product(int a, const Operand& oa, int ka, int b, int b2, const Operand& ob, int kb, int col, int n, int a_z = 0, int b_z = 0,
+               int a_step = 0, int b_step = 0, int part = 2) {
+    const int64_t K = oa.extent(ka);
+    static const int order[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};  // what is left out is below 2^-24
+    const int group = col >= 128 ? 1 : 0;
+    for (int i = P == 3 && part != 1 ? 0 : 5; i < (part == 0 ? (P == 3 ? 5 : 0) : 6); ++i) {
+      TORCH_CHECK(t.n_seg < kMaxSegs, "dense: too many segments");
+      Seg& s = t.seg[t.n_seg++];
+      s.a = (int8_t)a; s.b = (int8_t)b; s.b2 = (int8_t)(b2 < 0 ? b : b2);
+      s.a_mn = oa.mn(ka); s.b_mn = ob.mn(kb);
+      s.group = (int8_t)group;
+      s.spread = i == 5;
+      s.col = (int16_t)col; s.n = (int16_t)n;
+      s.za = a_z + order[i][0]; s.zb = b_z + order[i][1];
+      s.za_step = a_step; s.zb_step = b_step;
+      s.nk = (int)((K + BK - 1) / BK);
+      s.b2_off = b2 < 0 ? n / 2 : 0;
+      s.idesc = idesc16(bf16, s.a_mn, s.b_mn, n);
+      if (s.spread) t.main_nk[group] = s.nk;
+    }
+  }
+};
+
+// Plain product into `out` [batches][M][N].  256 columns a tile when that fills the GPU; the contraction axis is split over
+// several tiles (partials added in order by a second kernel) when there are fewer tiles than SMs and the axis is long, and
+// for float32 so that no accumulator takes more than 32 instructions of the large partial product.
+template <typename T, int BN, int STAGES, int ACC>
+void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
+  set_tiles(pl.t, M, N, BN, batches, 1);
+  const int tiles = pl.t.total, nk = pl.t.main_nk[0], kb = nk * pl.t.n_seg;
+  int splits = 1;
+  if (tiles < sm_count()) splits = std::max(1, std::min({2 * sm_count() / tiles, kb / 8, nk, 64}));
+  if (ACC > 1) splits = std::max(splits, (nk + 8 * ACC - 1) / (8 * ACC));
+  if (splits == 1) {
+    typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
+    run_dense<BN, STAGES, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);
+    return;
+  }
+  set_tiles(pl.t, M, N, BN, batches, splits);
+  const int64_t n = batches * M * N;
+  Tensor part = at::empty({splits, n}, out.options().dtype(at::kFloat));
+  typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n, 1.f};
+  run_dense<BN, STAGES, EpiStore<float, BN, ACC>>(pl.maps, pl.t, ep, st);
+  split_sum_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(part.data_ptr<float>(), splits, n, n, (T*)out.data_ptr());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// The number of columns has to be known when the segments are written: this is the rule.
+int store_bn(int P, int64_t batches, int64_t M, int64_t N) {
+  return P == 1 && batches * ((M + BM - 1) / BM) * ((N + 255) / 256) >= sm_count() ? 256 : 128;
+}
+void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
+  auto go = [&](auto v) {
+    using T = decltype(v);
+    if constexpr (sizeof(T) == 4) store_product<T, 128, 6, 4>(pl, out, batches, M, N, st);
+    else if (bn == 256) store_product<T, 256, 4, 1>(pl, out, batches, M, N, st);
+    else store_product<T, 128, 6, 1>(pl, out, batches, M, N, st);
+  };
+  if (out.scalar_type() == at::kFloat) go(float{});
+  else if (out.scalar_type() == at::kHalf) go(__half{});
+  else go(__nv_bfloat16{});
+}
+
+void check_ff(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
+  for (const Tensor* t : {&x, &wg, &wu, &wd})
+    TORCH_CHECK(t->is_cuda() && t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->dim() == 2,
+                "gated_ff: matrices of one type on one CUDA device");
+  TORCH_CHECK(x.scalar_type() == at::kFloat || x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16,
+              "gated_ff: float32, float16 or bfloat16");
+  TORCH_CHECK(wg.size(0) == x.size(1) && wu.sizes() == wg.sizes() && wd.size(0) == wg.size(1), "gated_ff: shapes do not fit");
+  TORCH_CHECK(act == kSilu || act == kGelu, "gated_ff: unknown activation");
+  TORCH_CHECK(x.size(0) < (1ll << 31) && x.size(1) >= 1 && wg.size(1) >= 1 && wd.size(1) >= 1, "gated_ff: sizes out of range");
+}
+
+}  // namespace
+
+Tensor gated_ff_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
+  check_ff(x, wg, wu, wd, act);
+  c10::cuda::CUDAGuard guard(x.device());
+  const int64_t M = x.size(0), H = wg.size(1), N = wd.size(1);
+  Tensor y = at::empty({M, N}, x.options());
+  if (M == 0) return y;
+  auto st = at::cuda::getCurrentCUDAStream();
+  const int P = planes_of(x);
+  const bool bf16 = x.scalar_type() != at::kHalf;
+  Operand ox = operand(x, st), og = operand(wg, st), ou = operand(wu, st), od = operand(wd, st);
+  if (og.rowmajor != ou.rowmajor) ou = operand(og.rowmajor ? wu.contiguous() : wu.t().contiguous().t(), st);
+  Operand oh = intermediate(M, H, P, x);
+  {
+    Plan pl(P, bf16);
+    const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou);
+    auto go = [&](auto v, auto bn_tag) {
+      using T = decltype(v);
+      constexpr int BN = decltype(bn_tag)::value;
+      pl.product(a, ox, 1, b, b2, og, 0, 0, BN);
+      set_tiles(pl.t, M, H, BN / 2, 1, 1);
+      typename EpiGated<T, BN>::Params ep{oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act};
+      run_dense<BN, BN == 256 ? 4 : 6, EpiGated<T, BN>>(pl.maps, pl.t, ep, st);
+    };
+    auto wide = [&](auto v) {
+      if constexpr (sizeof(v) == 2)
+        if (((M + BM - 1) / BM) * ((H + 127) / 128) >= sm_count()) return go(v, std::integral_constant<int, 256>{});
+      go(v, std::integral_constant<int, 128>{});
+    };
+    if (P == 3) wide(float{});
+    else if (bf16) wide(__nv_bfloat16{});
+    else wide(__half{});
+  }
+  Plan pl(P, bf16);
+  const int bn = store_bn(P, 1, M, N);
+  const int a = pl.map(oh), b = pl.map(od);
+  pl.product(a, oh, 1, b, -1, od, 0, 0, bn);
+  store_any(pl, bn, y, 1, M, N, st);
+  return y;
+}
+
+// which: bit 0 dx, bit 1 dWg and dWu, bit 2 dWd; the others come back empty.
+std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy, const Tensor& x, const Tensor& wg, const Tensor& wu,
+                                                        const Tensor& wd, int64_t act, int64_t which) {
+  check_ff(x, wg, wu, wd, act);
+  const int64_t M = x.size(0), K = x.size(1), H = wg.size(1), N = wd.size(1);
+  TORCH_CHECK(dy.device() == x.device() && dy.scalar_type() == x.scalar_type() && dy.dim() == 2 && dy.size(0) == M && dy.size(1) == N,
+              "gated_ff: dy does not fit");
+  c10::cuda::CUDAGuard guard(x.device());
+  auto st = at::cuda::getCurrentCUDAStream();
+  Tensor dx = at::empty({which & 1 ? M : 0, K}, x.options()), dgu = at::empty({2, which & 2 ? K : 0, H}, x.options()),
+         dwd = at::empty({which & 4 ? H : 0, N}, x.options());
+  if (M == 0 || (which & 7) == 0) {
+    dgu.zero_();
+    dwd.zero_();
+    return {dx, dgu.select(0, 0), dgu.select(0, 1), dwd};
+  }
+  const int P = planes_of(x);
+  const bool bf16 = x.scalar_type() != at::kHalf;
+  Operand ox = operand(x, st), og = operand(wg, st), ou = operand(wu, st), od = operand(wd, st), oy = operand(dy, st);
+  if (og.rowmajor != ou.rowmajor) ou = operand(og.rowmajor ? wu.contiguous() : wu.t().contiguous().t(), st);
+  Operand oe = intermediate(M, H, P, x, 2), oh = intermediate(M, H, P, x);  // dg then du; h
+  {
+    Plan pl(P, bf16);
+    const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou), a3 = pl.map(oy), b3 = pl.map(od);
+    pl.product(a, ox, 1, b, b2, og, 0, 0, 128);
+    pl.product(a3, oy, 1, b3, -1, od, 1, 128, 64);
+    set_tiles(pl.t, M, H, 64, 1, 1);
+    auto go = [&](auto v) {
+      using T = decltype(v);
+      uint16_t* e = (uint16_t*)oe.keep.data_ptr();
+      typename EpiGatedGrad<T>::Params ep{e, e + P * oe.s.plane, oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act};
+      run_dense<128, 6, EpiGatedGrad<T>>(pl.maps, pl.t, ep, st);
+    };
+    if (P == 3) go(float{});
+    else if (bf16) go(__nv_bfloat16{});
+    else go(__half{});
+  }
+  if (which & 1) {
+    Plan pl(P, bf16);
+    const int bn = store_bn(P, 1, M, K);
+    const int a = pl.map(oe), b = pl.map(og), c = pl.map(ou);
+    for (int part = 0; part < 2; ++part) {
+      pl.product(a, oe, 1, b, -1, og, 1, 0, bn, 0, 0, 0, 0, part);
+      pl.product(a, oe, 1, c, -1, ou, 1, 0, bn, P, 0, 0, 0, part);
+    }
+    store_any(pl, bn, dx, 1, M, K, st);
+  }
+  if (which & 2) {
+    Plan pl(P, bf16);
+    const int bn = store_bn(P, 2, K, H);
+    const int a = pl.map(ox), b = pl.map(oe);
+    pl.product(a, ox, 0, b, -1, oe, 0, 0, bn, 0, 0, 0, P);
+    store_any(pl, bn, dgu, 2, K, H, st);
+  }
+  if (which & 4) {
+    Plan pl(P, bf16);
+    const int bn = store_bn(P, 1, H, N);
+    const int a = pl.map(oh), b = pl.map(oy);
+    pl.product(a, oh, 0, b, -1, oy, 0, 0, bn);
+    store_any(pl, bn, dwd, 1, H, N, st);
+  }
+  return {dx, dgu.select(0, 0), dgu.select(0, 1), dwd};
+}
+
+// Reads (and clears) the error word of this file's kernels: 0 = no bounded wait expired since the last call.
+int64_t gated_ff_error_status(const Tensor& like) {
+  c10::cuda::CUDAGuard guard(like.device());
+  int v = 0, zero = 0;
+  C10_CUDA_CHECK(cudaMemcpyFromSymbol(&v, dense::error_word, sizeof(int)));
+  if (v != 0) C10_CUDA_CHECK(cudaMemcpyToSymbol(dense::error_word, &zero, sizeof(int)));
+  return v;
+}
+
+}  // namespace nva
+
+TORCH_LIBRARY_FRAGMENT(nvalchemi, m) {
+  m.def("gated_ff_fwd(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> Tensor", &nva::gated_ff_fwd);
+  m.def("gated_ff_bwd(Tensor dy, Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act, int which) -> (Tensor, Tensor, Tensor, Tensor)", &nva::gated_ff_bwd);
+  m.def("gated_ff_error_status(Tensor like) -> int", &nva::gated_ff_error_status);
+}

@@ -2,8 +2,10 @@
 """Model wrappers implementing the ``BaseModelMixin`` contract."""
 from nvalchemi_toolkit_b200.models.base import BaseModelMixin, ModelConfig, NeighborConfig, NeighborListFormat
 from nvalchemi_toolkit_b200.models.demo import DemoModel, DemoModelWrapper
+from nvalchemi_toolkit_b200.models.layers import GatedBlock, GatedFeedForward, LayerNorm
 
-__all__ = ["BaseModelMixin", "ModelConfig", "NeighborConfig", "NeighborListFormat", "DemoModel", "DemoModelWrapper"]
+__all__ = ["BaseModelMixin", "ModelConfig", "NeighborConfig", "NeighborListFormat", "DemoModel", "DemoModelWrapper", "GatedBlock",
+           "GatedFeedForward", "LayerNorm"]
 
 
 def __getattr__(name: str):

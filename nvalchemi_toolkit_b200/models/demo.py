@@ -6,6 +6,8 @@ an atomic-number embedding ``Embedding(100, H, padding_idx=0, max_norm=1)``, a c
 ``Linear(3,H) + LayerNorm + SiLU``, a joint MLP, and a per-atom energy projection summed per graph;
 forces are ``-dE/dr`` by autograd.  The model is not physical (it is not translation invariant); it
 exists to exercise the data, dynamics and hook layers cheaply on CPU and GPU.
+
+``gated_hidden > 0`` adds this package's pre-norm gated block (``models/layers.py``) of that hidden width after the joint MLP.
 """
 from __future__ import annotations
 
@@ -15,22 +17,25 @@ import torch
 from torch import nn
 
 from nvalchemi_toolkit_b200.models.base import BaseModelMixin, ModelConfig
+from nvalchemi_toolkit_b200.models.layers import GatedBlock
 
 
 class DemoModel(nn.Module):
-    def __init__(self, hidden_dim: int = 64) -> None:
+    def __init__(self, hidden_dim: int = 64, gated_hidden: int = 0) -> None:
         super().__init__()
-        self.hidden_dim = hidden_dim
+        self.hidden_dim, self.gated_hidden = hidden_dim, gated_hidden
         self.embedding = nn.Embedding(100, hidden_dim, padding_idx=0, max_norm=1.0)
         self.coord_embedding = nn.Sequential(nn.Linear(3, hidden_dim, bias=False), nn.LayerNorm(hidden_dim), nn.SiLU())
         self.joint_mlp = nn.Sequential(nn.Linear(2 * hidden_dim, hidden_dim), nn.LayerNorm(hidden_dim), nn.SiLU(),
                                        nn.Linear(hidden_dim, hidden_dim), nn.LayerNorm(hidden_dim), nn.SiLU())
         self.projection = nn.Linear(hidden_dim, 1, bias=False)
+        self.gated_block = GatedBlock(hidden_dim, gated_hidden) if gated_hidden else None
 
     def node_embeddings(self, atomic_numbers: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         z = self.embedding(atomic_numbers.long())
         c = self.coord_embedding(positions)
-        return self.joint_mlp(torch.cat([z, c], dim=-1))
+        h = self.joint_mlp(torch.cat([z, c], dim=-1))
+        return h if self.gated_block is None else self.gated_block(h)
 
     def forward(self, atomic_numbers: torch.Tensor, positions: torch.Tensor, batch_idx: torch.Tensor,
                 num_graphs: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -44,9 +49,9 @@ class DemoModel(nn.Module):
 class DemoModelWrapper(nn.Module, BaseModelMixin):
     """``BaseModelMixin`` adapter around :class:`DemoModel` (energy, autograd forces, embeddings)."""
 
-    def __init__(self, model: DemoModel | None = None, hidden_dim: int = 64) -> None:
+    def __init__(self, model: DemoModel | None = None, hidden_dim: int = 64, gated_hidden: int = 0) -> None:
         super().__init__()
-        self.model = model if model is not None else DemoModel(hidden_dim)
+        self.model = model if model is not None else DemoModel(hidden_dim, gated_hidden)
         self.model_config = ModelConfig(
             outputs=frozenset({"energy", "forces"}), autograd_outputs=frozenset({"forces"}),
             autograd_inputs=frozenset({"positions"}), supports_pbc=False, needs_pbc=False, neighbor_config=None,
@@ -89,7 +94,10 @@ class DemoModelWrapper(nn.Module, BaseModelMixin):
         return self.adapt_output(out, data)
 
     def checkpoint_spec(self) -> dict:
-        return {"cls": "nvalchemi_toolkit_b200.models.demo.DemoModelWrapper", "config": {"hidden_dim": self.model.hidden_dim}}
+        config = {"hidden_dim": self.model.hidden_dim}
+        if getattr(self.model, "gated_hidden", 0):
+            config["gated_hidden"] = self.model.gated_hidden
+        return {"cls": "nvalchemi_toolkit_b200.models.demo.DemoModelWrapper", "config": config}
 
     def distribution_spec(self, strategy: Any = None) -> Any:
         from nvalchemi_toolkit_b200.distributed.spec import SPEC_DEMO

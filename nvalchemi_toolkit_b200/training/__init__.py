@@ -6,7 +6,7 @@ from nvalchemi_toolkit_b200.training.losses import (
     ForceHuberLoss, ForceL2NormLoss, ForceMSELoss, LinearWeight, PiecewiseWeight, StressHuberLoss, StressMSELoss,
     as_composed_loss, assemble_loss_targets, compute_supervised_loss, loss_target_keys,
 )
-from nvalchemi_toolkit_b200.training.optimizers import OptimizerConfig
+from nvalchemi_toolkit_b200.training.optimizers import Muon, OptimizerConfig
 from nvalchemi_toolkit_b200.training.strategy import TrainingStrategy, default_training_fn
 from nvalchemi_toolkit_b200.training.validation import ValidationConfig, ValidationLoop
 
@@ -22,7 +22,7 @@ from nvalchemi_toolkit_b200.training.runtime import (configure_dataloader, confi
                                                      move_to_devices, train_configured_models)
 from nvalchemi_toolkit_b200.training.validation import BatchValidationCallback
 
-__all__ = ["TrainingStage", "TrainingStrategy", "default_training_fn", "OptimizerConfig", "ValidationConfig",
+__all__ = ["TrainingStage", "TrainingStrategy", "default_training_fn", "Muon", "OptimizerConfig", "ValidationConfig",
            "ValidationLoop", "BaseLossFunction", "ComposedLossFunction", "EnergyMSELoss", "EnergyMAELoss",
            "EnergyHuberLoss", "ForceMSELoss", "ForceHuberLoss", "ForceL2NormLoss", "StressMSELoss", "StressHuberLoss",
            "ConstantWeight", "LinearWeight", "CosineWeight", "PiecewiseWeight", "as_composed_loss", "assemble_loss_targets",

@@ -28,6 +28,97 @@ def check_kwargs(cls: Any, kwargs: Mapping[str, Any], label: str) -> None:
         raise ValueError(f"{label} {getattr(cls, '__name__', cls)} does not accept {unknown}; accepted: {accepted}")
 
 
+class Muon(torch.optim.Optimizer):
+    """Momentum whose matrix updates are orthogonalised by Newton-Schulz products (``ops.orthogonalize.newton_schulz``).
+
+    For a parameter with two axes or more (its last two are the matrix, the others a batch: MACE's stacked ``[l, C, C]`` channel
+    mixes are ``l`` matrices)::
+
+        buf <- momentum * buf + grad;   u = grad + momentum * buf  (nesterov)  or  buf
+        p   <- p * (1 - lr * weight_decay) - lr * 0.2 * sqrt(max(m, n)) * newton_schulz(u)
+
+    The factor gives an update of the root mean square size of an AdamW step, so ``lr`` and ``weight_decay`` are AdamW's.
+    Parameters with fewer axes, matrices with a side of one, and groups with ``orthogonalize=False`` (embedding tables, for
+    instance, by a ``ParamGroupSpec``) take AdamW steps with ``betas`` and ``adam_eps``.  Matrices of one shape are
+    orthogonalised together, one call for all of them."""
+
+    def __init__(self, params: Any, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+                 ns_steps: int = 5, betas: tuple[float, float] = (0.9, 0.999), adam_eps: float = 1e-8, orthogonalize: bool = True) -> None:
+        if not lr >= 0.0:
+            raise ValueError(f"Muon: lr must not be negative, got {lr}")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"Muon: momentum must lie in [0, 1), got {momentum}")
+        if not weight_decay >= 0.0:
+            raise ValueError(f"Muon: weight_decay must not be negative, got {weight_decay}")
+        if not all(0.0 <= b < 1.0 for b in betas) or not adam_eps > 0.0:
+            raise ValueError(f"Muon: betas must lie in [0, 1) and adam_eps be positive, got {betas}, {adam_eps}")
+        if int(ns_steps) != ns_steps or ns_steps < 1:
+            raise ValueError(f"Muon: ns_steps must be a positive whole number, got {ns_steps}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=int(ns_steps),
+                                      betas=tuple(betas), adam_eps=adam_eps, orthogonalize=orthogonalize))
+
+    @staticmethod
+    def _is_matrix(p: torch.Tensor) -> bool:
+        return p.dim() >= 2 and min(p.shape[-2:]) > 1
+
+    @torch.no_grad()
+    def step(self, closure: Callable[[], Any] | None = None) -> Any:
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            by_shape: dict[tuple, list[torch.Tensor]] = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse or p.is_complex():
+                    raise RuntimeError("Muon: sparse gradients and complex parameters are not supported")
+                if group["orthogonalize"] and self._is_matrix(p):
+                    by_shape.setdefault((tuple(p.shape[-2:]), p.dtype, p.device), []).append(p)
+                else:
+                    self._adam_step(p, group)
+            for (shape, _, _), ps in by_shape.items():
+                self._matrix_step(ps, shape, group)
+        return loss
+
+    def _matrix_step(self, ps: list[torch.Tensor], shape: tuple[int, int], group: dict[str, Any]) -> None:
+        from nvalchemi_toolkit_b200.ops.orthogonalize import newton_schulz
+
+        grads = [p.grad for p in ps]
+        bufs = [self.state[p].setdefault("momentum_buffer", torch.zeros_like(p, memory_format=torch.preserve_format)) for p in ps]
+        torch._foreach_mul_(bufs, group["momentum"])
+        torch._foreach_add_(bufs, grads)
+        updates = torch._foreach_add(grads, bufs, alpha=group["momentum"]) if group["nesterov"] else bufs
+        stacked = torch.cat([u.reshape(-1, *shape) for u in updates])
+        if stacked.dtype == torch.float64:
+            stacked = stacked.float()
+        o = newton_schulz(stacked, steps=group["ns_steps"])
+        scale = 0.2 * max(shape) ** 0.5
+        if group["weight_decay"]:
+            torch._foreach_mul_(ps, 1.0 - group["lr"] * group["weight_decay"])
+        row = 0
+        for p in ps:
+            count = p.numel() // (shape[0] * shape[1])
+            p.add_(o[row: row + count].reshape(p.shape).to(p.dtype), alpha=-group["lr"] * scale)
+            row += count
+
+    def _adam_step(self, p: torch.Tensor, group: dict[str, Any]) -> None:
+        st = self.state[p]
+        if "exp_avg" not in st:
+            st["adam_step"] = 0
+            st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+        b1, b2 = group["betas"]
+        st["adam_step"] += 1
+        st["exp_avg"].lerp_(p.grad, 1 - b1)
+        st["exp_avg_sq"].mul_(b2).addcmul_(p.grad, p.grad, value=1 - b2)
+        denom = (st["exp_avg_sq"] / (1 - b2 ** st["adam_step"])).sqrt_().add_(group["adam_eps"])
+        if group["weight_decay"]:
+            p.mul_(1.0 - group["lr"] * group["weight_decay"])
+        p.addcdiv_(st["exp_avg"], denom, value=-group["lr"] / (1 - b1 ** st["adam_step"]))
+
+
 class ParamGroupSpec(BaseModel):
     """Parameters whose qualified name matches ``pattern`` (``re.search``) form a group with their own optimiser options,
     e.g. ``ParamGroupSpec(pattern=r"bias$|norm", options={"weight_decay": 0.0})`` or a smaller ``lr`` for a pretrained trunk.

@@ -248,38 +248,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(slot));
 
+  // The segment is copied out of the parameters once: the compiler may not keep what it read there over an asm statement that
+  // clobbers memory, and both loops below would wait for constant loads before every instruction (43 % of the tensor pipe).
   if (warp == 0) {
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      for (int i = blockIdx.x; i < t.total && ok; i += gridDim.x) {
-        const TileAt at = tile_at(t, i);
-        for (int sg = 0; sg < t.n_seg && ok; ++sg) {
-          const Seg& s = t.seg[sg];
-          const int lo = split_at(s.nk, at.split, t.splits), hi = split_at(s.nk, at.split + 1, t.splits);
-          const int chunks = s.n / 64, half = (chunks + 1) / 2, m0 = at.m * BM, n0 = at.n * t.bn;
-          const int za = s.za + at.batch * s.za_step, zb = s.zb + at.batch * s.zb_step;
-          for (int kb = lo; kb < hi; ++kb, ++it) {
-            const int st = it % STAGES, k0 = kb * BK;
-            if (!mbar_wait(empty(st), ((it / STAGES) & 1) ^ 1, err, 11)) { ok = false; break; }
-            mbar_expect_tx(full(st), (uint32_t)(BM / 64 + chunks) * kChunk);
-            const uint32_t dst = base + st * STAGE;
-#pragma unroll
-            for (int c = 0; c < BM / 64; ++c) {
-              const int mn = m0 + 64 * c;
-              tma_load_3d(dst + c * kChunk, &maps.m[s.a], s.a_mn ? mn : k0, s.a_mn ? k0 : mn, za, full(st));
-            }
-            for (int c = 0; c < chunks; ++c) {
-              const bool second = c >= half;
-              const int mn = n0 + 64 * (second ? c - half : c) + (second ? s.b2_off : 0);
-              tma_load_3d(dst + (BM / 64 + c) * kChunk, &maps.m[second ? s.b2 : s.b], s.b_mn ? mn : k0, s.b_mn ? k0 : mn, zb, full(st));
-            }
-          }
+    // lane c loads chunk c of a stage: the first two are A's, the others B's
+    int it = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; i < t.total && ok; i += gridDim.x) {
+      const TileAt at = tile_at(t, i);
+      for (int sg = 0; sg < t.n_seg && ok; ++sg) {
+        const Seg s = t.seg[sg];
+        const int lo = split_at(s.nk, at.split, t.splits), hi = split_at(s.nk, at.split + 1, t.splits);
+        const int chunks = s.n / 64, half = (chunks + 1) / 2, c = lane - BM / 64;
+        const bool mine = c < chunks, is_a = c < 0, second = c >= half;
+        const CUtensorMap* const map = &maps.m[is_a ? s.a : second ? s.b2 : s.b];
+        const int mn = is_a ? at.m * BM + 64 * lane : at.n * t.bn + 64 * (second ? c - half : c) + (second ? s.b2_off : 0);
+        const int z = is_a ? s.za + at.batch * s.za_step : s.zb + at.batch * s.zb_step;
+        const bool mn_first = is_a ? s.a_mn : s.b_mn;
+        const uint32_t bytes = (uint32_t)(BM / 64 + chunks) * kChunk;
+        for (int kb = lo; kb < hi; ++kb, ++it) {
+          const int st = it % STAGES, k0 = kb * BK;
+          if (!mbar_wait(empty(st), ((it / STAGES) & 1) ^ 1, err, 11)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          if (lane == 0) mbar_expect_tx(full(st), bytes);
+          __syncwarp();
+          if (mine) tma_load_3d(base + st * STAGE + lane * kChunk, map, mn_first ? mn : k0, mn_first ? k0 : mn, z, full(st));
         }
       }
-      if (!ok)  // gave up: the copies in flight must have landed before the CTA's shared memory is given back
-        for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(full(j % STAGES), (j / STAGES) & 1, err, 14);
     }
+    if (!ok)  // gave up: the copies in flight must have landed before the CTA's shared memory is given back
+      for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(full(j % STAGES), (j / STAGES) & 1, err, 14);
   } else if (warp == 1) {
     if (lane == 0) {
       int it = 0, n_tile = 0;
@@ -291,21 +289,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         uint32_t started = 0;  // accumulators that hold something of this tile
         for (int sg = 0; sg < t.n_seg && ok; ++sg) {
-          const Seg& s = t.seg[sg];
+          const Seg s = t.seg[sg];
           const int lo = split_at(s.nk, at.split, t.splits), hi = split_at(s.nk, at.split + 1, t.splits);
+          const uint64_t da0 = desc16(base, s.a_mn), db0 = desc16(base + (BM / 64) * kChunk, s.b_mn);
+          const uint32_t ka = (s.a_mn ? 2048 : 32) >> 4, kb_step = (s.b_mn ? 2048 : 32) >> 4;
+          const uint32_t d0 = tmem + as * 256 + s.col;
           for (int kb = lo; kb < hi; ++kb, ++it) {
             const int st = it % STAGES;
             if (!mbar_wait(full(st), (it / STAGES) & 1, err, 13)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t sa = base + st * STAGE, sb = sa + (BM / 64) * kChunk;
+            const uint64_t da = da0 + (uint32_t)(st * (int)(STAGE >> 4)), db = db0 + (uint32_t)(st * (int)(STAGE >> 4));
             const int j = ACC > 1 && s.spread ? (kb - lo) % ACC : 0;
-            const uint32_t d = tmem + as * 256 + s.col + j * Epi::kStride, bit = 1u << (s.group * ACC + j);
-            const bool fresh = (started & bit) == 0;
+            const uint32_t d = d0 + j * Epi::kStride, bit = 1u << (s.group * ACC + j);
+            const uint32_t acc = (started & bit) != 0 ? 1u : 0u;
             started |= bit;
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              mma16(d, desc16(sa + k * (s.a_mn ? 2048 : 32), s.a_mn), desc16(sb + k * (s.b_mn ? 2048 : 32), s.b_mn), s.idesc,
-                    (fresh && k == 0) ? 0u : 1u);
+            for (int k = 0; k < BK / 16; ++k) mma16(d, da + k * ka, db + k * kb_step, s.idesc, k == 0 ? acc : 1u);
             umma_commit(empty(st));
           }
         }

@@ -53,16 +53,16 @@ struct EpiGram {
 #pragma unroll 1
     for (int cb = 0; cb < 2; ++cb) {
       const int c = half * 64 + cb * 32, n0 = at.n * 128 + c;
-      float v[32];
+      float v[32], dg = 0.f;
       tmem_ld32(tm + c, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         v[j] *= 1.f / kXScale;  // accumulated 2^24 A
-        if (row == n0 + j) {
-          if (row < t.M) p.diag[at.batch * (int64_t)t.M + row] = v[j] * (1.f / kXScale);
-          v[j] = 0.f;
-        }
+        const bool on = row == n0 + j;
+        dg = on ? v[j] : dg;
+        v[j] = on ? 0.f : v[j];
       }
+      if (row >= n0 && row < n0 + 32 && row < t.M) p.diag[at.batch * (int64_t)t.M + row] = dg * (1.f / kXScale);
       store_symmetric(stage, v, out, p.ld, t.M, row0, n0, at.m != at.n);
     }
   }
@@ -78,31 +78,28 @@ struct EpiPoly {
     const float* d = p.diag + at.batch * (int64_t)t.M;
     const int row = row0 + (threadIdx.x & 31);
     const float di = row < t.M ? d[row] : 0.f;
+    // every global load of a chunk is issued before anything is done with one: inside conditions they would wait for each
+    // other (15 us a launch that way)
 #pragma unroll 1
     for (int cb = 0; cb < 2; ++cb) {
-      const int c = half * 64 + cb * 32, n0 = at.n * 128 + c;
-      float v[32];
+      const int c = half * 64 + cb * 32, n0 = at.n * 128 + c, lane = threadIdx.x & 31;
+      uint4 raw[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)  // rows are padded to 8
+        raw[q] = row < t.M && n0 + 8 * q < t.M ? *reinterpret_cast<const uint4*>(r + (int64_t)row * p.ld + n0 + 8 * q) : make_uint4(0, 0, 0, 0);
+      const float dl = n0 + lane < t.M ? d[n0 + lane] : 0.f;
+      float v[32], dg = 0.f;
       tmem_ld32(tm + c, v);
-      if (row < t.M) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint4 raw = make_uint4(0, 0, 0, 0);
-          if (n0 + 8 * q < t.M) raw = *reinterpret_cast<const uint4*>(r + (int64_t)row * p.ld + n0 + 8 * q);  // rows are padded to 8
-          const __half* h = reinterpret_cast<const __half*>(&raw);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int j = 8 * q + k, col = n0 + j;
-            const float aa = v[j] * (1.f / (kXScale * kXScale)), rij = __half2float(h[k]) * (1.f / kXScale);
-            if (col == row) {
-              p.bdiag[at.batch * (int64_t)t.M + row] = p.b * di + p.c * (di * di + aa);
-              v[j] = 0.f;
-            } else {
-              const float dj = col < t.M ? __ldg(d + col) : 0.f;
-              v[j] = (p.b * rij + p.c * ((di + dj) * rij + aa)) * kBScale;
-            }
-          }
-        }
+      for (int j = 0; j < 32; ++j) {
+        const float aa = v[j] * (1.f / (kXScale * kXScale));
+        const float rij = __half2float(reinterpret_cast<const __half*>(raw)[j]) * (1.f / kXScale);
+        const float dj = __shfl_sync(0xffffffffu, dl, j);
+        const bool on = row == n0 + j;
+        dg = on ? aa : dg;
+        v[j] = on ? 0.f : (p.b * rij + p.c * ((di + dj) * rij + aa)) * kBScale;
       }
+      if (row >= n0 && row < n0 + 32 && row < t.M) p.bdiag[at.batch * (int64_t)t.M + row] = p.b * di + p.c * (di * di + dg);
       store_symmetric(stage, v, p.bo + at.batch * p.stride, p.ld, t.M, row0, n0, at.m != at.n);
     }
   }
@@ -131,26 +128,25 @@ struct EpiUpdate {
     for (int cb = 0; cb < BN / 64; ++cb) {
       const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c;
       if (n0 >= t.N) break;
+      const int64_t off = base + (int64_t)row * p.ld + n0;
+      float4 xs[8];
+      uint4 raw[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // rows are padded to 8
+        const bool in = row < t.M && n0 + 8 * q < t.N;
+        xs[2 * q] = in ? *reinterpret_cast<const float4*>(p.x + off + 8 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
+        xs[2 * q + 1] = in ? *reinterpret_cast<const float4*>(p.x + off + 8 * q + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        raw[q] = in && !p.two ? *reinterpret_cast<const uint4*>(p.xh + off + 8 * q) : make_uint4(0, 0, 0, 0);
+      }
+      const float bl = p.tall && n0 + (int)(threadIdx.x & 31) < t.N ? bd[n0 + (threadIdx.x & 31)] : 0.f;
       float v[32];
       tmem_ld32(tm + c, v);
-      if (row < t.M) {
-        const int64_t off = base + (int64_t)row * p.ld + n0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (n0 + 8 * q < t.N) {  // rows are padded to 8
-            const float4 x0 = *reinterpret_cast<const float4*>(p.x + off + 8 * q), x1 = *reinterpret_cast<const float4*>(p.x + off + 8 * q + 4);
-            const uint4 raw = *reinterpret_cast<const uint4*>(p.xh + off + 8 * q);
-            const __half* h = reinterpret_cast<const __half*>(&raw);
-            const float xs[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int j = 8 * q + k;
-              const float b = p.tall ? (n0 + j < t.N ? __ldg(bd + n0 + j) : 0.f) : bi;
-              const float xb = p.two ? xs[k] : __half2float(h[k]) * (1.f / kXScale);  // the X that the product read
-              v[j] = p.a * xs[k] + b * xb + v[j] * (1.f / (kXScale * kBScale));
-            }
-          }
-        }
+      for (int j = 0; j < 32; ++j) {
+        const float x = reinterpret_cast<const float*>(xs)[j];
+        const float b = p.tall ? __shfl_sync(0xffffffffu, bl, j) : bi;
+        const float xb = p.two ? x : __half2float(reinterpret_cast<const __half*>(raw)[j]) * (1.f / kXScale);  // what the product read
+        v[j] = p.a * x + b * xb + v[j] * (1.f / (kXScale * kBScale));
       }
       if (p.out != nullptr) {
         uint4 o[4];

@@ -15,10 +15,18 @@
 // over several tiles.
 //
 // One persistent CTA per SM: warp 0 loads tiles by TMA into a ring of stages, one lane of warp 1 issues tcgen05.mma
-// (M = 128, K = 16 per instruction), warps 2..9 are the epilogue.  The accumulator is double buffered (2 x 256 TMEM columns),
-// so the epilogue of a tile runs beside the products of the next one; products with several accumulators use all of the TMEM
-// for one tile (their six passes hide the epilogue less, but it is a tenth of them).  Every wait is bounded; on expiry the error word is
-// set, the roles leave their loops, the producer waits (bounded) for its copies in flight, and the TMEM is freed.
+// (K = 16 per instruction), warps 2..9 are the epilogue.  The accumulator is double buffered (2 x 256 TMEM columns), so the
+// epilogue of a tile runs beside the products of the next one; products with several accumulators use all of the TMEM for one
+// tile (their six passes hide the epilogue less, but it is a tenth of them).
+//
+// Tiles of more than 128 rows are worked on by pairs of CTAs (cta_group::2): 256 rows, each CTA holds its 128 rows of A, half
+// of the tile of B and 128 rows of the accumulator.  What bounds one CTA by itself is shared memory: at 128 x 256 a 64-wide
+// block writes 48 KB and reads 48 KB, at the 117 bytes a clock it reaches 450 ns (1370 TFLOP/s at 18944 x 4096 x 4096), while
+// the instructions need 320 ns; an instruction of 128 or 64 columns needs 195 ns whichever it is.  A pair writes 32 KB and reads
+// 32 KB per CTA.
+//
+// Every wait is bounded; on expiry the error word is set, the roles leave their loops, the producer waits (bounded) for its
+// copies in flight, and the TMEM is freed.
 #pragma once
 #include "common.cuh"
 #include "convert.cuh"
@@ -53,8 +61,9 @@ struct Seg {
 struct Tiles {
   int M, N;              // rows and columns of one output matrix
   int mt, nt, bn;        // tiles along each, columns of a tile
+  int bm;                // rows of a tile: 128, or 256 for a pair of CTAs
   int batches, splits, total;
-  int lower;             // 1: symmetric output, only tiles on and below the diagonal
+  int lower;             // symmetric output, only tiles that reach the diagonal or lie below it: bm / bn, else 0
   int n_seg;
   int main_nk[2];        // nk of the spread segments of each group
   Seg seg[kMaxSegs];
@@ -62,7 +71,7 @@ struct Tiles {
 
 struct alignas(64) Maps { CUtensorMap m[kMaxMaps]; };
 
-struct TileAt { int m, n, batch, split; };
+struct TileAt { int m, n, batch, split, seq; };  // seq: the CTA's how-manieth tile
 
 // The part of a segment's blocks that one of `splits` tiles of the same output takes.
 __device__ __forceinline__ int split_at(int nk, int split, int splits) { return (int)((int64_t)nk * split / splits); }
@@ -75,19 +84,21 @@ __device__ __forceinline__ int used_acc(const Tiles& t, const TileAt& at, int gr
 }
 
 // Tiles of eight row blocks run together, column by column, so that concurrent CTAs share operand tiles in the L2.
-__device__ __forceinline__ TileAt tile_at(const Tiles& t, int i) {
+__device__ __forceinline__ TileAt tile_at(const Tiles& t, int i, int seq) {
   TileAt r;
-  const int per = t.lower ? t.mt * (t.mt + 1) / 2 : t.mt * t.nt;
+  r.seq = seq;
+  const int per = t.lower ? t.lower * (t.mt * (t.mt + 1) / 2) : t.mt * t.nt;
   const int z = i / per;
-  int j = i - z * per;
+  const int j = i - z * per;
   r.batch = z % t.batches;
   r.split = z / t.batches;
-  if (t.lower) {  // square tiles: row m holds m + 1 of them
-    int m = (int)((sqrtf(8.f * (float)j + 1.f) - 1.f) * 0.5f);
-    while ((m + 1) * (m + 2) / 2 <= j) ++m;
-    while (m * (m + 1) / 2 > j) --m;
+  if (t.lower) {  // row m holds lower * (m + 1) tiles
+    const int k = j / t.lower;
+    int m = (int)((sqrtf(8.f * (float)k + 1.f) - 1.f) * 0.5f);
+    while ((m + 1) * (m + 2) / 2 <= k) ++m;
+    while (m * (m + 1) / 2 > k) --m;
     r.m = m;
-    r.n = j - m * (m + 1) / 2;
+    r.n = j - t.lower * (m * (m + 1) / 2);
     return r;
   }
   constexpr int G = 8;
@@ -98,11 +109,19 @@ __device__ __forceinline__ TileAt tile_at(const Tiles& t, int i) {
   return r;
 }
 
+// PAIR: the barrier may be the other CTA's (a shared::cluster address).
+template <bool PAIR>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
 }
 
 // 128-byte swizzle.  K-major: 8-row groups 1024 bytes apart.  MN-major: 8 contraction rows per 1024 bytes, 64-wide chunks of
@@ -111,21 +130,31 @@ __device__ __forceinline__ uint64_t desc16(uint32_t addr, bool mn) {
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)((mn ? kChunk : 0) >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-inline uint32_t idesc16(bool bf16, bool a_mn, bool b_mn, int n) {
+inline uint32_t idesc16(bool bf16, bool a_mn, bool b_mn, int n, int m) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma16(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
 }
 
-template <int BN> constexpr int stage_bytes() { return (BM / 64 + BN / 64) * kChunk; }
+// A stage of one CTA: 128 rows of A and the tile of B, or half of it in a pair.
+template <int BN, bool PAIR> constexpr int stage_bytes() { return (BM / 64 + BN / (PAIR ? 128 : 64)) * kChunk; }
+template <int BN, bool PAIR> constexpr int stage_count() { return 196608 / stage_bytes<BN, PAIR>(); }
 // ring + per-warp staging (32 rows of 128 bytes) + barriers, and slack for 1024-byte alignment
-template <int BN, int STAGES> constexpr int smem_bytes() { return 1024 + STAGES * stage_bytes<BN>() + kEpiWarps * 4096 + 256; }
+template <int BN, bool PAIR> constexpr int smem_bytes() { return 1024 + stage_count<BN, PAIR>() * stage_bytes<BN, PAIR>() + kEpiWarps * 4096 + 512; }
 
 // One warp's 32 rows x (SLOTS * 16) bytes from registers (lane = row) to global memory in whole row pieces: through shared
 // memory, 16-byte slots swizzled by row so that neither side has bank conflicts.  `cols_left`: elements of type T that exist
@@ -214,13 +243,18 @@ __device__ __forceinline__ void acc_ld32(uint32_t tm, float (&v)[32], int used) 
   }
 }
 
-// Epi::kAcc accumulators kStride columns apart, Epi::Params, Epi::run(params, tiles, tile, tmem (lane quarter added), first row of the warp, half, stage).
-template <int BN, int STAGES, typename Epi>
+// Epi::kAcc accumulators per column group, kStride columns apart; Epi::kLate: see below; Epi::Params; Epi::run(params, tiles,
+// tile, tmem (lane quarter added), first row of the warp, half, stage).
+//
+// kLate: a tile fills TMEM columns 0..383, group 0 in 0..255 and group 1 (whose segments come first) in the 128 columns after
+// those, in turns with the last 128, so that the next tile's group 1 is formed while the epilogue still reads this tile.
+template <int BN, bool PAIR, typename Epi>
 __global__ void __launch_bounds__(kThreads, 1)
     dense_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Tiles t, const __grid_constant__ typename Epi::Params ep) {
   extern __shared__ uint8_t smem_raw[];
-  constexpr uint32_t STAGE = stage_bytes<BN>();
-  constexpr int ACC = Epi::kAcc, BUFS = ACC == 1 ? 2 : 1;
+  constexpr int STAGES = stage_count<BN, PAIR>();
+  constexpr uint32_t STAGE = stage_bytes<BN, PAIR>();
+  constexpr int ACC = Epi::kAcc, BUFS = ACC == 1 && !Epi::kLate ? 2 : 1, CTAS = PAIR ? 2 : 1;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const generic = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bar0 = base + STAGES * STAGE + kEpiWarps * 4096;
@@ -230,20 +264,28 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto acc_empty = [&](int s) { return bar0 + 8u * (2 * STAGES + 2 + s); };
   const uint32_t slot = bar0 + 8u * (2 * STAGES + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const int first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
   int* const err = &error_word;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(acc_full(s), 1); mbar_init(acc_empty(s), kEpiWarps); }
+    for (int s = 0; s < 2; ++s) { mbar_init(acc_full(s), 1); mbar_init(acc_empty(s), kEpiWarps * CTAS); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the other CTA's barriers are ready
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(slot));
@@ -251,52 +293,72 @@ __global__ void __launch_bounds__(kThreads, 1)
   // The segment is copied out of the parameters once: the compiler may not keep what it read there over an asm statement that
   // clobbers memory, and both loops below would wait for constant loads before every instruction (43 % of the tensor pipe).
   if (warp == 0) {
-    // lane c loads chunk c of a stage: the first two are A's, the others B's
-    int it = 0;
-    bool ok = true;
-    for (int i = blockIdx.x; i < t.total && ok; i += gridDim.x) {
-      const TileAt at = tile_at(t, i);
-      for (int sg = 0; sg < t.n_seg && ok; ++sg) {
-        const Seg s = t.seg[sg];
-        const int lo = split_at(s.nk, at.split, t.splits), hi = split_at(s.nk, at.split + 1, t.splits);
-        const int chunks = s.n / 64, half = (chunks + 1) / 2, c = lane - BM / 64;
-        const bool mine = c < chunks, is_a = c < 0, second = c >= half;
-        const CUtensorMap* const map = &maps.m[is_a ? s.a : second ? s.b2 : s.b];
-        const int mn = is_a ? at.m * BM + 64 * lane : at.n * t.bn + 64 * (second ? c - half : c) + (second ? s.b2_off : 0);
-        const int z = is_a ? s.za + at.batch * s.za_step : s.zb + at.batch * s.zb_step;
-        const bool mn_first = is_a ? s.a_mn : s.b_mn;
-        const uint32_t bytes = (uint32_t)(BM / 64 + chunks) * kChunk;
-        for (int kb = lo; kb < hi; ++kb, ++it) {
-          const int st = it % STAGES, k0 = kb * BK;
-          if (!mbar_wait(empty(st), ((it / STAGES) & 1) ^ 1, err, 11)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          if (lane == 0) mbar_expect_tx(full(st), bytes);
-          __syncwarp();
-          if (mine) tma_load_3d(base + st * STAGE + lane * kChunk, map, mn_first ? mn : k0, mn_first ? k0 : mn, z, full(st));
-        }
-      }
-    }
-    if (!ok)  // gave up: the copies in flight must have landed before the CTA's shared memory is given back
-      for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j) mbar_wait(full(j % STAGES), (j / STAGES) & 1, err, 14);
-  } else if (warp == 1) {
     if (lane == 0) {
-      int it = 0, n_tile = 0;
+      int st = 0, seq = 0, issued = 0;
+      uint32_t phase = 1;
       bool ok = true;
-      for (int i = blockIdx.x; i < t.total && ok; i += gridDim.x, ++n_tile) {
-        const TileAt at = tile_at(t, i);
-        const int as = BUFS == 2 ? n_tile & 1 : 0;
-        if (!mbar_wait(acc_empty(as), ((n_tile / BUFS) & 1) ^ 1, err, 12)) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint32_t started = 0;  // accumulators that hold something of this tile
+      for (int i = first_tile; i < t.total && ok; i += tile_step, ++seq) {
+        const TileAt at = tile_at(t, i, seq);
         for (int sg = 0; sg < t.n_seg && ok; ++sg) {
           const Seg s = t.seg[sg];
           const int lo = split_at(s.nk, at.split, t.splits), hi = split_at(s.nk, at.split + 1, t.splits);
+          // chunks of B in this CTA; the tile's second half (b2) is the second CTA's, or the second half of this one's chunks
+          const int chunks = s.n / (64 * CTAS), half = PAIR ? 0 : (chunks + 1) / 2;
+          const CUtensorMap* const ma = &maps.m[s.a];
+          const CUtensorMap* const mb = &maps.m[PAIR && rank == 1 ? s.b2 : s.b];
+          const CUtensorMap* const mb2 = &maps.m[s.b2];
+          const int m0 = at.m * (BM * CTAS) + (int)rank * BM, n0 = at.n * t.bn + (PAIR && rank == 1 ? s.b2_off : 0), n2 = at.n * t.bn + s.b2_off;
+          const int za = s.za + at.batch * s.za_step, zb = s.zb + at.batch * s.zb_step;
+          const bool a_mn = s.a_mn, b_mn = s.b_mn;
+          const uint32_t bytes = (uint32_t)(BM / 64 + chunks) * kChunk * CTAS;
+          for (int kb = lo; kb < hi; ++kb) {
+            if (!mbar_wait(empty(st), phase, err, 11)) { ok = false; break; }
+            const uint32_t bar = PAIR ? map_to_rank(full(st), 0) : full(st);
+            if (rank == 0) mbar_expect_tx(full(st), bytes);
+            const uint32_t dst = base + st * STAGE;
+            const int k0 = kb * BK;
+#pragma unroll
+            for (int c = 0; c < BM / 64; ++c)
+              tma_load_3d<PAIR>(dst + c * kChunk, ma, a_mn ? m0 + 64 * c : k0, a_mn ? k0 : m0 + 64 * c, za, bar);
+#pragma unroll
+            for (int c = 0; c < BN / (64 * CTAS); ++c)
+              if (c < chunks) {
+                const bool second = !PAIR && c >= half;
+                const int mn = second ? n2 + 64 * (c - half) : n0 + 64 * c;
+                tma_load_3d<PAIR>(dst + (BM / 64 + c) * kChunk, second ? mb2 : mb, b_mn ? mn : k0, b_mn ? k0 : mn, zb, bar);
+              }
+            ++issued;
+            if (++st == STAGES) { st = 0; phase ^= 1; }
+          }
+        }
+      }
+      if (!ok && rank == 0)  // gave up: the copies in flight (both CTAs') must have landed before the shared memory is given back
+        for (int j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j) mbar_wait(full(j % STAGES), (j / STAGES) & 1, err, 14);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int st = 0, seq = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = first_tile; i < t.total && ok; i += tile_step, ++seq) {
+        const TileAt at = tile_at(t, i, seq);
+        const int as = BUFS == 2 ? seq & 1 : 0;
+        bool free = false;     // the epilogue has left this tile's accumulators
+        uint32_t started = 0;  // accumulators that hold something of this tile
+        for (int sg = 0; sg < t.n_seg && ok; ++sg) {
+          const Seg s = t.seg[sg];
+          if (!free && (!Epi::kLate || s.group == 0)) {
+            ok = mbar_wait_cluster(acc_empty(as), ((seq / BUFS) & 1) ^ 1, err, 12);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            free = true;
+          }
+          const int lo = split_at(s.nk, at.split, t.splits), hi = split_at(s.nk, at.split + 1, t.splits);
           const uint64_t da0 = desc16(base, s.a_mn), db0 = desc16(base + (BM / 64) * kChunk, s.b_mn);
           const uint32_t ka = (s.a_mn ? 2048 : 32) >> 4, kb_step = (s.b_mn ? 2048 : 32) >> 4;
-          const uint32_t d0 = tmem + as * 256 + s.col;
-          for (int kb = lo; kb < hi; ++kb, ++it) {
-            const int st = it % STAGES;
-            if (!mbar_wait(full(st), (it / STAGES) & 1, err, 13)) { ok = false; break; }
+          const uint32_t d0 = tmem + as * 256 + s.col + (Epi::kLate && s.group == 1 ? (seq & 1) * 128 : 0);
+          for (int kb = lo; kb < hi; ++kb) {
+            if (!mbar_wait_cluster(full(st), phase, err, 13)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t da = da0 + (uint32_t)(st * (int)(STAGE >> 4)), db = db0 + (uint32_t)(st * (int)(STAGE >> 4));
             const int j = ACC > 1 && s.spread ? (kb - lo) % ACC : 0;
@@ -304,37 +366,48 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t acc = (started & bit) != 0 ? 1u : 0u;
             started |= bit;
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) mma16(d, da + k * ka, db + k * kb_step, s.idesc, k == 0 ? acc : 1u);
-            umma_commit(empty(st));
+            for (int k = 0; k < BK / 16; ++k) mma16<PAIR>(d, da + k * ka, db + k * kb_step, s.idesc, k == 0 ? acc : 1u);
+            if constexpr (PAIR) umma_commit_pair(empty(st));
+            else umma_commit(empty(st));
+            if (++st == STAGES) { st = 0; phase ^= 1; }
           }
         }
-        umma_commit(acc_full(as));
+        if constexpr (PAIR) umma_commit_pair(acc_full(as));
+        else umma_commit(acc_full(as));
       }
     }
   } else {
     const int w = warp - 2, q = warp & 3, half = w >> 2;  // q: the TMEM lanes this warp may read
     uint4* const stage = reinterpret_cast<uint4*>(generic + STAGES * STAGE + w * 4096);
-    int n_tile = 0;
-    for (int i = blockIdx.x; i < t.total; i += gridDim.x, ++n_tile) {
-      const TileAt at = tile_at(t, i);
-      const int as = BUFS == 2 ? n_tile & 1 : 0;
-      if (!mbar_wait(acc_full(as), (n_tile / BUFS) & 1, err, 15)) break;
+    int seq = 0;
+    for (int i = first_tile; i < t.total; i += tile_step, ++seq) {
+      const TileAt at = tile_at(t, i, seq);
+      const int as = BUFS == 2 ? seq & 1 : 0;
+      if (!mbar_wait_cluster(acc_full(as), (seq / BUFS) & 1, err, 15)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      Epi::run(ep, t, at, tmem + as * 256 + ((uint32_t)(q * 32) << 16), at.m * BM + q * 32, half, stage);
+      Epi::run(ep, t, at, tmem + as * 256 + ((uint32_t)(q * 32) << 16), at.m * (BM * CTAS) + (int)rank * BM + q * 32, half, stage);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty(as));
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster(map_to_rank(acc_empty(as), 0));
+        else mbar_arrive(acc_empty(as));
+      }
     }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if constexpr (PAIR) cluster_sync();  // nothing of the pair is under way any more
+  if (warp == 1) {
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
 }
 
 // out[batch][split][M][N] = alpha * acc, as T.
 template <typename T, int BN, int ACC>
 struct EpiStore {
   static constexpr int kAcc = ACC, kStride = BN;
+  static constexpr bool kLate = false;
   static_assert(ACC == 1 || ACC * BN <= 512, "dense: accumulators exceed the TMEM");
   struct Params { T* out; int64_t ld, batch_stride, split_stride; float alpha; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
@@ -400,23 +473,54 @@ inline int sm_count() {
   return n;
 }
 
-inline void set_tiles(Tiles& t, int64_t M, int64_t N, int bn, int64_t batches, int splits, bool lower = false) {
+// More than one block of 128 rows: pairs of CTAs (their tile of 256 rows costs less than two of 128).
+inline bool use_pair(int64_t M) { return M > BM; }
+
+// In a pair every CTA holds half of the tile of B, so n / 2 of each segment has to be a multiple of 64.
+inline void set_tiles(Tiles& t, int64_t M, int64_t N, int bn, int64_t batches, int splits, bool lower = false, bool pair_ok = true) {
   t.M = (int)M; t.N = (int)N; t.bn = bn;
-  t.mt = (int)((M + BM - 1) / BM); t.nt = (int)((N + bn - 1) / bn);
-  t.batches = (int)batches; t.splits = splits; t.lower = lower ? 1 : 0;
-  const int64_t per = lower ? (int64_t)t.mt * (t.mt + 1) / 2 : (int64_t)t.mt * t.nt;
+  t.bm = pair_ok && use_pair(M) ? 2 * BM : BM;
+  t.mt = (int)((M + t.bm - 1) / t.bm); t.nt = (int)((N + bn - 1) / bn);
+  t.batches = (int)batches; t.splits = splits; t.lower = lower ? t.bm / bn : 0;
+  TORCH_CHECK(!lower || (t.lower >= 1 && t.bm % bn == 0), "dense: symmetric tiles do not fit");
+  const int64_t per = lower ? (int64_t)t.lower * ((int64_t)t.mt * (t.mt + 1) / 2) : (int64_t)t.mt * t.nt;
   TORCH_CHECK(per * batches * splits < (1ll << 31), "dense: too many tiles");
   t.total = (int)(per * batches * splits);
 }
+// Tiles that run at the same time.
+inline int slots(const Tiles& t) { return t.bm == BM ? sm_count() : sm_count() / 2; }
 
-template <int BN, int STAGES, typename Epi>
-void run_dense(const Maps& maps, const Tiles& t, const typename Epi::Params& ep, cudaStream_t st) {
-  constexpr int smem = smem_bytes<BN, STAGES>();
+template <int BN, bool PAIR, typename Epi>
+void launch_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cudaStream_t st) {
+  constexpr int smem = smem_bytes<BN, PAIR>();
   static_assert(smem <= 227 * 1024, "dense: stages exceed shared memory");
+  for (int i = 0; i < t.n_seg; ++i) t.seg[i].idesc = (t.seg[i].idesc & 0xFFFFFFu) | (uint32_t)((PAIR ? 2 * BM : BM) >> 4) << 24;
   // set on every call: the attribute belongs to the current device's context
-  C10_CUDA_CHECK(cudaFuncSetAttribute(dense_kernel<BN, STAGES, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  dense_kernel<BN, STAGES, Epi><<<std::min(t.total, sm_count()), kThreads, smem, st>>>(maps, t, ep);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  C10_CUDA_CHECK(cudaFuncSetAttribute(dense_kernel<BN, PAIR, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(std::min(t.total, slots(t)) * (PAIR ? 2 : 1)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, dense_kernel<BN, PAIR, Epi>, maps, t, ep));
+}
+template <int BN, typename Epi, bool PAIR_OK = true>
+void run_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cudaStream_t st) {
+  if (t.bm == BM) {
+    if constexpr (BN == 256 && !Epi::kLate) {
+      TORCH_CHECK(false, "dense: 256-column tiles are for pairs");
+    } else {
+      launch_dense<BN, false, Epi>(maps, t, ep, st);
+    }
+  } else if constexpr (PAIR_OK) {
+    for (int i = 0; i < t.n_seg; ++i) TORCH_CHECK(t.seg[i].n % 128 == 0, "dense: a segment too narrow for a pair");
+    launch_dense<BN, true, Epi>(maps, t, ep, st);
+  }
 }
 
 }  // namespace dense

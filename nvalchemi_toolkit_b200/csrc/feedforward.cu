@@ -91,6 +91,7 @@ __device__ __forceinline__ void store32(uint4* stage, float (&v)[32], void* dst,
 template <typename T, int BN>
 struct EpiGated {
   static constexpr int kAcc = sizeof(T) == 4 ? 512 / BN : 1, kStride = BN;
+  static constexpr bool kLate = false;
   struct Params { void* h; int64_t ld, plane; int act; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
                                              uint4* stage) {
@@ -108,25 +109,32 @@ struct EpiGated {
   }
 };
 
-// Columns [0, 64): g, [64, 128): u, [128, 192): dh of 64 columns.
+// Of HC columns of h: g in accumulator columns [0, HC), u in [HC, 2 HC), dh after those.  16 bits: 128 columns, dh in turns in
+// two places (see dense_kernel); float32: 64 columns, two accumulators each.
 template <typename T>
 struct EpiGatedGrad {
+  static constexpr int kHc = sizeof(T) == 4 ? 64 : 128;
   static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1, kStride = 192;
+  static constexpr bool kLate = sizeof(T) == 2;
   struct Params { void *dg, *du, *h; int64_t ld, plane; int act; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
                                              uint4* stage) {
-    const int c = half * 32, n0 = at.n * 64 + c;
-    float g[32], u[32], d[32];
-    const int used = used_acc<kAcc>(t, at, 0);
-    acc_ld32<kAcc, kStride>(tm + c, g, used);
-    acc_ld32<kAcc, kStride>(tm + 64 + c, u, used);
-    acc_ld32<kAcc, kStride>(tm + 128 + c, d, used_acc<kAcc>(t, at, 1));
-    if (p.act == kSilu) gate_grad32<sizeof(T) == 4, kSilu>(g, u, d);
-    else gate_grad32<sizeof(T) == 4, kGelu>(g, u, d);
-    const int64_t off = (int64_t)row0 * p.ld + n0;
-    store32<T>(stage, g, p.dg, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
-    store32<T>(stage, d, p.du, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
-    store32<T>(stage, u, p.h, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
+    const int used = used_acc<kAcc>(t, at, 0), used1 = used_acc<kAcc>(t, at, 1);
+    const uint32_t td = tm + 2 * kHc + (kLate ? (at.seq & 1) * 128 : 0);
+#pragma unroll 1
+    for (int cb = 0; cb < kHc / 64; ++cb) {
+      const int c = half * (kHc / 2) + cb * 32, n0 = at.n * kHc + c;
+      float g[32], u[32], d[32];
+      acc_ld32<kAcc, kStride>(tm + c, g, used);
+      acc_ld32<kAcc, kStride>(tm + kHc + c, u, used);
+      acc_ld32<kAcc, kStride>(td + c, d, used1);
+      if (p.act == kSilu) gate_grad32<sizeof(T) == 4, kSilu>(g, u, d);
+      else gate_grad32<sizeof(T) == 4, kGelu>(g, u, d);
+      const int64_t off = (int64_t)row0 * p.ld + n0;
+      store32<T>(stage, g, p.dg, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
+      store32<T>(stage, d, p.du, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
+      store32<T>(stage, u, p.h, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
+    }
   }
 };
 
@@ -219,10 +227,9 @@ struct Plan {
   // a[.., k] . b[.., k]; ka / kb: the axis of each logical matrix that is contracted; b2 < 0: both halves from b.
   // part 0: the small partial products of float32 operands (added first), 1: the large one, 2: both.
   void product(int a, const Operand& oa, int ka, int b, int b2, const Operand& ob, int kb, int col, int n, int a_z = 0, int b_z = 0,
-               int a_step = 0, int b_step = 0, int part = 2) {
+               int a_step = 0, int b_step = 0, int part = 2, int group = 0) {
     const int64_t K = oa.extent(ka);
     static const int order[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};  // what is left out is below 2^-24
-    const int group = col >= 128 ? 1 : 0;
     for (int i = P == 3 && part != 1 ? 0 : 5; i < (part == 0 ? (P == 3 ? 5 : 0) : 6); ++i) {
       TORCH_CHECK(t.n_seg < kMaxSegs, "dense: too many segments");
       Seg& s = t.seg[t.n_seg++];
@@ -235,46 +242,46 @@ struct Plan {
       s.za_step = a_step; s.zb_step = b_step;
       s.nk = (int)((K + BK - 1) / BK);
       s.b2_off = b2 < 0 ? n / 2 : 0;
-      s.idesc = idesc16(bf16, s.a_mn, s.b_mn, n);
+      s.idesc = idesc16(bf16, s.a_mn, s.b_mn, n, BM);
       if (s.spread) t.main_nk[group] = s.nk;
     }
   }
 };
 
-// Plain product into `out` [batches][M][N].  256 columns a tile when that fills the GPU; the contraction axis is split over
-// several tiles (partials added in order by a second kernel) when there are fewer tiles than SMs and the axis is long, and
-// for float32 so that no accumulator takes more than 32 instructions of the large partial product.
-template <typename T, int BN, int STAGES, int ACC>
+// Plain product into `out` [batches][M][N].  The contraction axis is split over several tiles (partials added in order by a
+// second kernel) when there are fewer tiles than the GPU runs at a time and the axis is long, and for float32 so that no
+// accumulator takes more than 32 instructions of the large partial product.
+template <typename T, int BN, int ACC>
 void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   set_tiles(pl.t, M, N, BN, batches, 1);
-  const int tiles = pl.t.total, nk = pl.t.main_nk[0], kb = nk * pl.t.n_seg;
+  const int tiles = pl.t.total, nk = pl.t.main_nk[0], kb = nk * pl.t.n_seg, at_once = slots(pl.t);
   int splits = 1;
-  if (tiles < sm_count()) splits = std::max(1, std::min({2 * sm_count() / tiles, kb / 8, nk, 64}));
+  if (tiles < at_once) splits = std::max(1, std::min({2 * at_once / tiles, kb / 8, nk, 64}));
   if (ACC > 1) splits = std::max(splits, (nk + 8 * ACC - 1) / (8 * ACC));
   if (splits == 1) {
     typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
-    run_dense<BN, STAGES, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);
+    run_dense<BN, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);
     return;
   }
   set_tiles(pl.t, M, N, BN, batches, splits);
   const int64_t n = batches * M * N;
   Tensor part = at::empty({splits, n}, out.options().dtype(at::kFloat));
   typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n, 1.f};
-  run_dense<BN, STAGES, EpiStore<float, BN, ACC>>(pl.maps, pl.t, ep, st);
+  run_dense<BN, EpiStore<float, BN, ACC>>(pl.maps, pl.t, ep, st);
   split_sum_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(part.data_ptr<float>(), splits, n, n, (T*)out.data_ptr());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// The number of columns has to be known when the segments are written: this is the rule.
+// Columns of a tile: 256 (less shared-memory traffic per product) where that still gives every pair of CTAs a tile.
 int store_bn(int P, int64_t batches, int64_t M, int64_t N) {
-  return P == 1 && batches * ((M + BM - 1) / BM) * ((N + 255) / 256) >= sm_count() ? 256 : 128;
+  return P == 1 && use_pair(M) && batches * ((M + 2 * BM - 1) / (2 * BM)) * ((N + 255) / 256) >= sm_count() / 2 ? 256 : 128;
 }
 void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   auto go = [&](auto v) {
     using T = decltype(v);
-    if constexpr (sizeof(T) == 4) store_product<T, 128, 6, 4>(pl, out, batches, M, N, st);
-    else if (bn == 256) store_product<T, 256, 4, 1>(pl, out, batches, M, N, st);
-    else store_product<T, 128, 6, 1>(pl, out, batches, M, N, st);
+    if constexpr (sizeof(T) == 4) store_product<T, 128, 4>(pl, out, batches, M, N, st);
+    else if (bn == 256) store_product<T, 256, 1>(pl, out, batches, M, N, st);
+    else store_product<T, 128, 1>(pl, out, batches, M, N, st);
   };
   if (out.scalar_type() == at::kFloat) go(float{});
   else if (out.scalar_type() == at::kHalf) go(__half{});
@@ -315,11 +322,11 @@ Tensor gated_ff_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const T
       pl.product(a, ox, 1, b, b2, og, 0, 0, BN);
       set_tiles(pl.t, M, H, BN / 2, 1, 1);
       typename EpiGated<T, BN>::Params ep{oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act};
-      run_dense<BN, BN == 256 ? 4 : 6, EpiGated<T, BN>>(pl.maps, pl.t, ep, st);
+      run_dense<BN, EpiGated<T, BN>>(pl.maps, pl.t, ep, st);
     };
     auto wide = [&](auto v) {
       if constexpr (sizeof(v) == 2)
-        if (((M + BM - 1) / BM) * ((H + 127) / 128) >= sm_count()) return go(v, std::integral_constant<int, 256>{});
+        if (store_bn(P, 1, M, 2 * H) == 256) return go(v, std::integral_constant<int, 256>{});
       go(v, std::integral_constant<int, 128>{});
     };
     if (P == 3) wide(float{});
@@ -358,14 +365,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy, const 
   {
     Plan pl(P, bf16);
     const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou), a3 = pl.map(oy), b3 = pl.map(od);
-    pl.product(a, ox, 1, b, b2, og, 0, 0, 128);
-    pl.product(a3, oy, 1, b3, -1, od, 1, 128, 64);
-    set_tiles(pl.t, M, H, 64, 1, 1);
+    const int hc = P == 3 ? 64 : 128;
+    pl.product(a3, oy, 1, b3, -1, od, 1, 2 * hc, hc, 0, 0, 0, 0, 2, 1);
+    pl.product(a, ox, 1, b, b2, og, 0, 0, 2 * hc);
+    set_tiles(pl.t, M, H, hc, 1, 1, false, P == 1);  // 64 columns of dh are too few for a pair
     auto go = [&](auto v) {
       using T = decltype(v);
       uint16_t* e = (uint16_t*)oe.keep.data_ptr();
       typename EpiGatedGrad<T>::Params ep{e, e + P * oe.s.plane, oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act};
-      run_dense<128, 6, EpiGatedGrad<T>>(pl.maps, pl.t, ep, st);
+      run_dense<2 * EpiGatedGrad<T>::kHc, EpiGatedGrad<T>, sizeof(T) == 2>(pl.maps, pl.t, ep, st);
     };
     if (P == 3) go(float{});
     else if (bf16) go(__nv_bfloat16{});

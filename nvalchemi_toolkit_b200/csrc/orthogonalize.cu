@@ -43,16 +43,18 @@ __device__ __forceinline__ void store_symmetric(uint4* stage, const float (&v)[3
 }
 
 // R = A without its diagonal (times 2^12), diag(A).
+template <int BN>
 struct EpiGram {
-  static constexpr int kAcc = 1, kStride = 128;
+  static constexpr int kAcc = 1, kStride = BN;
+  static constexpr bool kLate = false;
   struct Params { __half* r; float* diag; int64_t ld, stride; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
                                              uint4* stage) {
     __half* out = p.r + at.batch * p.stride;
     const int row = row0 + (threadIdx.x & 31);
 #pragma unroll 1
-    for (int cb = 0; cb < 2; ++cb) {
-      const int c = half * 64 + cb * 32, n0 = at.n * 128 + c;
+    for (int cb = 0; cb < BN / 64; ++cb) {
+      const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c;
       float v[32], dg = 0.f;
       tmem_ld32(tm + c, v);
 #pragma unroll
@@ -63,14 +65,16 @@ struct EpiGram {
         v[j] = on ? 0.f : v[j];
       }
       if (row >= n0 && row < n0 + 32 && row < t.M) p.diag[at.batch * (int64_t)t.M + row] = dg * (1.f / kXScale);
-      store_symmetric(stage, v, out, p.ld, t.M, row0, n0, at.m != at.n);
+      store_symmetric(stage, v, out, p.ld, t.M, row0, n0, at.n < t.lower * at.m);
     }
   }
 };
 
 // B = b A + c A A, split the same way.
+template <int BN>
 struct EpiPoly {
-  static constexpr int kAcc = 1, kStride = 128;
+  static constexpr int kAcc = 1, kStride = BN;
+  static constexpr bool kLate = false;
   struct Params { const __half* r; const float* diag; __half* bo; float* bdiag; int64_t ld, stride; float b, c; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
                                              uint4* stage) {
@@ -81,8 +85,8 @@ struct EpiPoly {
     // every global load of a chunk is issued before anything is done with one: inside conditions they would wait for each
     // other (15 us a launch that way)
 #pragma unroll 1
-    for (int cb = 0; cb < 2; ++cb) {
-      const int c = half * 64 + cb * 32, n0 = at.n * 128 + c, lane = threadIdx.x & 31;
+    for (int cb = 0; cb < BN / 64; ++cb) {
+      const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c, lane = threadIdx.x & 31;
       uint4 raw[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q)  // rows are padded to 8
@@ -100,7 +104,7 @@ struct EpiPoly {
         v[j] = on ? 0.f : (p.b * rij + p.c * ((di + dj) * rij + aa)) * kBScale;
       }
       if (row >= n0 && row < n0 + 32 && row < t.M) p.bdiag[at.batch * (int64_t)t.M + row] = p.b * di + p.c * (di * di + dg);
-      store_symmetric(stage, v, p.bo + at.batch * p.stride, p.ld, t.M, row0, n0, at.m != at.n);
+      store_symmetric(stage, v, p.bo + at.batch * p.stride, p.ld, t.M, row0, n0, at.n < t.lower * at.m);
     }
   }
 };
@@ -109,6 +113,7 @@ struct EpiPoly {
 template <int BN>
 struct EpiUpdate {
   static constexpr int kAcc = 1, kStride = BN;
+  static constexpr bool kLate = false;
   struct Params {
     const float* x; const __half* xh; const float* bdiag;  // xh: high parts; low parts `plane` further (two != 0)
     float* x_out; __half* xh_out; __nv_bfloat16* out;  // out != null: last step
@@ -232,7 +237,7 @@ void add_segment(Tiles& t, int a, bool a_mn, int b, bool b_mn, int64_t K, int n,
   s.za_step = s.zb_step = 1;
   s.nk = (int)((K + BK - 1) / BK);
   s.b2_off = n / 2;
-  s.idesc = idesc16(false, a_mn, b_mn, n);
+  s.idesc = idesc16(false, a_mn, b_mn, n, BM);
   t.main_nk[0] = s.nk;
 }
 
@@ -274,7 +279,10 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
   float *ad = diag.data_ptr<float>(), *bd = ad + batch * r;
   auto stored_x = [&](int which) { return Stored{xh0 + which * planes * plane, n, m, ld, planes * batch, m * ld}; };
   const Stored sr{rp, r, r, rld, batch, r * rld}, sb{bp, r, r, rld, batch, r * rld};
-  const int bn = batch * ((m + BM - 1) / BM) * ((n + 255) / 256) >= sm_count() ? 256 : 128;
+  // columns of a tile: 256 where that still gives every pair of CTAs a tile
+  auto wide = [&](int64_t rows, int64_t tiles) { return use_pair(rows) && tiles >= sm_count() / 2; };
+  const int64_t rt = (r + 255) / 256;
+  const int bn = wide(m, batch * ((m + 255) / 256) * ((n + 255) / 256)) ? 256 : 128, sbn = wide(r, batch * (rt * (rt + 1) / 2)) ? 256 : 128;
   for (int64_t i = 0; i < steps; ++i) {
     const int cur = (int)(i & 1);
     {
@@ -282,17 +290,19 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
       Tiles t{};
       put_map(maps, 0, stored_x(cur));
       for (int k = planes == 2 ? 0 : 2; k < 3; ++k)  // low . high, high . low, high . high
-        add_segment(t, 0, tall, 0, tall, tall ? m : n, 128, k == 0 ? (int)batch : 0, k == 1 ? (int)batch : 0);
-      set_tiles(t, r, r, 128, batch, 1, true);
-      run_dense<128, 6, EpiGram>(maps, t, {rp, ad, rld, r * rld}, st);
+        add_segment(t, 0, tall, 0, tall, tall ? m : n, sbn, k == 0 ? (int)batch : 0, k == 1 ? (int)batch : 0);
+      set_tiles(t, r, r, sbn, batch, 1, true);
+      if (sbn == 256) run_dense<256, EpiGram<256>>(maps, t, {rp, ad, rld, r * rld}, st);
+      else run_dense<128, EpiGram<128>>(maps, t, {rp, ad, rld, r * rld}, st);
     }
     {
       Maps maps;
       Tiles t{};
       put_map(maps, 0, sr);
-      add_segment(t, 0, false, 0, false, r, 128);
-      set_tiles(t, r, r, 128, batch, 1, true);
-      run_dense<128, 6, EpiPoly>(maps, t, {rp, ad, bp, bd, rld, r * rld, (float)b, (float)c}, st);
+      add_segment(t, 0, false, 0, false, r, sbn);
+      set_tiles(t, r, r, sbn, batch, 1, true);
+      if (sbn == 256) run_dense<256, EpiPoly<256>>(maps, t, {rp, ad, bp, bd, rld, r * rld, (float)b, (float)c}, st);
+      else run_dense<128, EpiPoly<128>>(maps, t, {rp, ad, bp, bd, rld, r * rld, (float)b, (float)c}, st);
     }
     Maps maps;
     Tiles t{};
@@ -306,7 +316,7 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
                                         xh0 + (1 - cur) * planes * plane,
                                         i + 1 == steps ? (__nv_bfloat16*)out.data_ptr() : nullptr, ld, m * ld, m * n, plane, tall ? 1 : 0, (int)r, planes - 1,
                                         (float)a};
-      run_dense<BN, BN == 256 ? 4 : 6, EpiUpdate<BN>>(maps, t, ep, st);
+      run_dense<BN, EpiUpdate<BN>>(maps, t, ep, st);
     };
     if (bn == 256) update(std::integral_constant<int, 256>{});
     else update(std::integral_constant<int, 128>{});

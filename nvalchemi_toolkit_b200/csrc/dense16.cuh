@@ -41,7 +41,7 @@ namespace dense {
 
 constexpr int BM = 128, BK = 64, kChunk = 64 * 64 * 2;  // a chunk: 64 x 64 16-bit values, one TMA box
 constexpr int kMaxSegs = 12, kMaxMaps = 6, kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
 
 static __device__ int error_word;
 
@@ -69,12 +69,14 @@ struct Tiles {
   Seg seg[kMaxSegs];
 };
 
-struct alignas(64) Maps { CUtensorMap m[kMaxMaps]; };
+struct alignas(64) Maps { CUtensorMap m[kMaxMaps]; int n = 0; };
 
 struct TileAt { int m, n, batch, split, seq; };  // seq: the CTA's how-manieth tile
 
 // The part of a segment's blocks that one of `splits` tiles of the same output takes.
-__device__ __forceinline__ int split_at(int nk, int split, int splits) { return (int)((int64_t)nk * split / splits); }
+__device__ __forceinline__ int split_at(int nk, int split, int splits) {
+  return splits == 1 ? nk * split : (int)((int64_t)nk * split / splits);
+}
 // How many of a group's ACC accumulators the tile's products have written.
 template <int ACC>
 __device__ __forceinline__ int used_acc(const Tiles& t, const TileAt& at, int group) {
@@ -126,11 +128,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 
 // 128-byte swizzle.  K-major: 8-row groups 1024 bytes apart.  MN-major: 8 contraction rows per 1024 bytes, 64-wide chunks of
 // the M / N axis one TMA box (8192 bytes) apart.
-__device__ __forceinline__ uint64_t desc16(uint32_t addr, bool mn) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)((mn ? kChunk : 0) >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+__device__ __forceinline__ uint64_t desc16(uint32_t addr, bool mn, uint32_t chunk = kChunk) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)((mn ? chunk : 0) >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-inline uint32_t idesc16(bool bf16, bool a_mn, bool b_mn, int n, int m) {
+__host__ __device__ constexpr uint32_t idesc16(bool bf16, bool a_mn, bool b_mn, int n, int m) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
@@ -168,24 +170,53 @@ __device__ __forceinline__ void store_piece(uint4* stage, const uint4 (&v)[SLOTS
 #pragma unroll
   for (int j = 0; j < SLOTS; ++j) stage[lane * SLOTS + (j ^ (lane & (SLOTS - 1)))] = v[j];
   __syncwarp();
-  const int slot = lane % SLOTS, r0 = lane / SLOTS;
+  if (vec_ok && cols_left >= SLOTS * PER) {
+    const int slot = lane % SLOTS, r0 = lane / SLOTS;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int r = i * RPI + r0;
+      if (r < rows_left)
+        *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + slot * PER) = stage[r * SLOTS + (slot ^ (r & (SLOTS - 1)))];
+    }
+  } else {  // rows off the 16-byte boundaries, or the last columns: a row at a time, an element a lane
+    const T* const e = reinterpret_cast<const T*>(stage);
+    constexpr int W = SLOTS * PER;  // 32 or 64 elements
+#pragma unroll
+    for (int c = 0; c < W; c += 32) {
+      const int j = c + lane, slot = j / PER, k = j % PER;
+#pragma unroll 8
+      for (int r = 0; r < 32; ++r)
+        if (r < rows_left && j < cols_left) dst[(int64_t)r * ld + j] = e[(r * SLOTS + (slot ^ (r & (SLOTS - 1)))) * PER + k];
+    }
+  }
+  __syncwarp();
+}
+
+// The way back: 32 rows x (SLOTS * 16) bytes from global memory in whole row pieces (rows on 16-byte boundaries), then, through
+// shared memory, a row a lane.  Row by row from global memory every lane would touch a cache line of its own: 4000 clocks for
+// three pieces of eight warps.
+template <typename T, int SLOTS>
+__device__ __forceinline__ void fetch_piece(uint4 (&raw)[SLOTS], const T* src, int64_t ld, int rows_left, int cols_left) {
+  const int lane = threadIdx.x & 31, slot = lane % SLOTS, r0 = lane / SLOTS;
+  constexpr int PER = 16 / (int)sizeof(T), RPI = 32 / SLOTS;
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
     const int r = i * RPI + r0;
-    const uint4 val = stage[r * SLOTS + (slot ^ (r & (SLOTS - 1)))];
-    const int left = cols_left - slot * PER;
-    if (r < rows_left && left > 0) {
-      T* p = dst + (int64_t)r * ld + slot * PER;
-      if (vec_ok && left >= PER) {
-        *reinterpret_cast<uint4*>(p) = val;
-      } else {
-        const T* e = reinterpret_cast<const T*>(&val);
-#pragma unroll
-        for (int k = 0; k < PER; ++k)
-          if (k < left) p[k] = e[k];
-      }
-    }
+    raw[i] = r < rows_left && slot * PER < cols_left ? *reinterpret_cast<const uint4*>(src + (int64_t)r * ld + slot * PER) : make_uint4(0, 0, 0, 0);
   }
+}
+template <int SLOTS>
+__device__ __forceinline__ void turn_piece(uint4* stage, uint4 (&raw)[SLOTS]) {
+  const int lane = threadIdx.x & 31, slot = lane % SLOTS, r0 = lane / SLOTS;
+  constexpr int RPI = 32 / SLOTS;
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) {
+    const int r = i * RPI + r0;
+    stage[r * SLOTS + (slot ^ (r & (SLOTS - 1)))] = raw[i];
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < SLOTS; ++j) raw[j] = stage[lane * SLOTS + (j ^ (lane & (SLOTS - 1)))];
   __syncwarp();
 }
 
@@ -243,8 +274,9 @@ __device__ __forceinline__ void acc_ld32(uint32_t tm, float (&v)[32], int used) 
   }
 }
 
-// Epi::kAcc accumulators per column group, kStride columns apart; Epi::kLate: see below; Epi::Params; Epi::run(params, tiles,
-// tile, tmem (lane quarter added), first row of the warp, half, stage).
+// Epi::kAcc accumulators per column group, kStride columns apart; Epi::kLate: see below; Epi::Params; Epi::Pre: what
+// Epi::prefetch(params, tiles, tile, first row of the warp, half, pre) reads before the tile's products are done;
+// Epi::run(params, tiles, tile, tmem (lane quarter added), first row, half, stage, pre).
 //
 // kLate: a tile fills TMEM columns 0..383, group 0 in 0..255 and group 1 (whose segments come first) in the 128 columns after
 // those, in turns with the last 128, so that the next tile's group 1 is formed while the epilogue still reads this tile.
@@ -268,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
   int* const err = &error_word;
 
+  if (warp == 0 && lane < maps.n) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.m[lane]) : "memory");
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(acc_full(s), 1); mbar_init(acc_empty(s), kEpiWarps * CTAS); }
@@ -382,10 +415,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int seq = 0;
     for (int i = first_tile; i < t.total; i += tile_step, ++seq) {
       const TileAt at = tile_at(t, i, seq);
-      const int as = BUFS == 2 ? seq & 1 : 0;
+      const int as = BUFS == 2 ? seq & 1 : 0, row0 = at.m * (BM * CTAS) + (int)rank * BM + q * 32;
+      typename Epi::Pre pre;
+      Epi::prefetch(ep, t, at, row0, half, pre);
       if (!mbar_wait_cluster(acc_full(as), (seq / BUFS) & 1, err, 15)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      Epi::run(ep, t, at, tmem + as * 256 + ((uint32_t)(q * 32) << 16), at.m * (BM * CTAS) + (int)rank * BM + q * 32, half, stage);
+      Epi::run(ep, t, at, tmem + as * 256 + ((uint32_t)(q * 32) << 16), row0, half, stage, pre);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
@@ -403,15 +438,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// For epilogues that read nothing.
+struct NoPrefetch {
+  struct Pre {};
+  template <typename P>
+  static __device__ __forceinline__ void prefetch(const P&, const Tiles&, const TileAt&, int, int, Pre&) {}
+};
+
 // out[batch][split][M][N] = alpha * acc, as T.
 template <typename T, int BN, int ACC>
-struct EpiStore {
+struct EpiStore : NoPrefetch {
   static constexpr int kAcc = ACC, kStride = BN;
   static constexpr bool kLate = false;
   static_assert(ACC == 1 || ACC * BN <= 512, "dense: accumulators exceed the TMEM");
   struct Params { T* out; int64_t ld, batch_stride, split_stride; float alpha; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
-                                             uint4* stage) {
+                                             uint4* stage, Pre&) {
     T* out = p.out + at.batch * p.batch_stride + at.split * p.split_stride;
     const bool vec_ok = p.ld % (16 / (int)sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     const int used = used_acc<ACC>(t, at, 0);
@@ -449,6 +491,7 @@ struct Stored {
 
 inline void put_map(Maps& maps, int i, const Stored& s) {
   TORCH_CHECK(i < kMaxMaps, "dense: too many tensor maps");
+  maps.n = std::max(maps.n, i + 1);
   const int64_t ld = s.outer > 1 ? s.ld : (s.inner + 7) / 8 * 8;
   const int64_t plane = s.planes > 1 ? s.plane : ld * s.outer;
   TORCH_CHECK(s.inner > 0 && s.outer > 0 && ld % 8 == 0 && plane % 8 == 0 && (reinterpret_cast<uintptr_t>(s.p) & 15) == 0,
@@ -487,6 +530,14 @@ inline void set_tiles(Tiles& t, int64_t M, int64_t N, int bn, int64_t batches, i
   TORCH_CHECK(per * batches * splits < (1ll << 31), "dense: too many tiles");
   t.total = (int)(per * batches * splits);
 }
+// Columns of a pair's tile, 256 or 128, by the number of tiles of each kind: the wide one takes less shared-memory traffic per
+// product (320 ns against 2 x 225 ns per 64-wide block), the narrow one may fill the last round of the GPU better.
+inline int pick_bn(int64_t tiles256, int64_t tiles128) {
+  const int64_t pairs = sm_count() / 2;
+  const double wide = (double)((tiles256 + pairs - 1) / pairs), narrow = 0.7 * (double)((tiles128 + pairs - 1) / pairs);
+  return wide <= narrow ? 256 : 128;
+}
+
 // Tiles that run at the same time.
 inline int slots(const Tiles& t) { return t.bm == BM ? sm_count() : sm_count() / 2; }
 

@@ -89,12 +89,12 @@ __device__ __forceinline__ void store32(uint4* stage, float (&v)[32], void* dst,
 
 // Columns [0, BN/2) of the accumulator: g, [BN/2, BN): u, both of the same BN/2 columns of h.
 template <typename T, int BN>
-struct EpiGated {
+struct EpiGated : NoPrefetch {
   static constexpr int kAcc = sizeof(T) == 4 ? 512 / BN : 1, kStride = BN;
   static constexpr bool kLate = false;
   struct Params { void* h; int64_t ld, plane; int act; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
-                                             uint4* stage) {
+                                             uint4* stage, Pre&) {
     const int used = used_acc<kAcc>(t, at, 0);
 #pragma unroll 1
     for (int cb = 0; cb < BN / 128; ++cb) {
@@ -112,13 +112,13 @@ struct EpiGated {
 // Of HC columns of h: g in accumulator columns [0, HC), u in [HC, 2 HC), dh after those.  16 bits: 128 columns, dh in turns in
 // two places (see dense_kernel); float32: 64 columns, two accumulators each.
 template <typename T>
-struct EpiGatedGrad {
+struct EpiGatedGrad : NoPrefetch {
   static constexpr int kHc = sizeof(T) == 4 ? 64 : 128;
   static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1, kStride = 192;
   static constexpr bool kLate = sizeof(T) == 2;
   struct Params { void *dg, *du, *h; int64_t ld, plane; int act; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
-                                             uint4* stage) {
+                                             uint4* stage, Pre&) {
     const int used = used_acc<kAcc>(t, at, 0), used1 = used_acc<kAcc>(t, at, 1);
     const uint32_t td = tm + 2 * kHc + (kLate ? (at.seq & 1) * 128 : 0);
 #pragma unroll 1
@@ -272,9 +272,11 @@ void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N,
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// Columns of a tile: 256 (less shared-memory traffic per product) where that still gives every pair of CTAs a tile.
+// Columns of a tile of an M x N product.
 int store_bn(int P, int64_t batches, int64_t M, int64_t N) {
-  return P == 1 && use_pair(M) && batches * ((M + 2 * BM - 1) / (2 * BM)) * ((N + 255) / 256) >= sm_count() / 2 ? 256 : 128;
+  if (P != 1 || !use_pair(M)) return 128;
+  const int64_t rows = batches * ((M + 2 * BM - 1) / (2 * BM));
+  return pick_bn(rows * ((N + 255) / 256), rows * ((N + 127) / 128));
 }
 void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   auto go = [&](auto v) {

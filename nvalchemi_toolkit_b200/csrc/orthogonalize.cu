@@ -44,12 +44,12 @@ __device__ __forceinline__ void store_symmetric(uint4* stage, const float (&v)[3
 
 // R = A without its diagonal (times 2^12), diag(A).
 template <int BN>
-struct EpiGram {
+struct EpiGram : NoPrefetch {
   static constexpr int kAcc = 1, kStride = BN;
   static constexpr bool kLate = false;
   struct Params { __half* r; float* diag; int64_t ld, stride; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
-                                             uint4* stage) {
+                                             uint4* stage, Pre&) {
     __half* out = p.r + at.batch * p.stride;
     const int row = row0 + (threadIdx.x & 31);
 #pragma unroll 1
@@ -76,22 +76,28 @@ struct EpiPoly {
   static constexpr int kAcc = 1, kStride = BN;
   static constexpr bool kLate = false;
   struct Params { const __half* r; const float* diag; __half* bo; float* bdiag; int64_t ld, stride; float b, c; };
+  struct Pre { uint4 raw[4]; float dl; };  // 32 columns of R (rows are padded to 8), and of the diagonal
+  static __device__ __forceinline__ void fetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int n0, Pre& pre) {
+    const int lane = threadIdx.x & 31;
+    fetch_piece<__half, 4>(pre.raw, p.r + at.batch * p.stride + (int64_t)row0 * p.ld + n0, p.ld, t.M - row0, t.M - n0);
+    pre.dl = n0 + lane < t.M ? p.diag[at.batch * (int64_t)t.M + n0 + lane] : 0.f;
+  }
+  static __device__ __forceinline__ void prefetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int half, Pre& pre) {
+    fetch(p, t, at, row0, at.n * BN + half * (BN / 2), pre);
+  }
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
-                                             uint4* stage) {
-    const __half* r = p.r + at.batch * p.stride;
-    const float* d = p.diag + at.batch * (int64_t)t.M;
+                                             uint4* stage, Pre& pre) {
     const int row = row0 + (threadIdx.x & 31);
-    const float di = row < t.M ? d[row] : 0.f;
-    // every global load of a chunk is issued before anything is done with one: inside conditions they would wait for each
-    // other (15 us a launch that way)
+    const float di = row < t.M ? p.diag[at.batch * (int64_t)t.M + row] : 0.f;
 #pragma unroll 1
     for (int cb = 0; cb < BN / 64; ++cb) {
-      const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c, lane = threadIdx.x & 31;
+      const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c;
+      turn_piece<4>(stage, pre.raw);
       uint4 raw[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)  // rows are padded to 8
-        raw[q] = row < t.M && n0 + 8 * q < t.M ? *reinterpret_cast<const uint4*>(r + (int64_t)row * p.ld + n0 + 8 * q) : make_uint4(0, 0, 0, 0);
-      const float dl = n0 + lane < t.M ? d[n0 + lane] : 0.f;
+      for (int q = 0; q < 4; ++q) raw[q] = pre.raw[q];
+      const float dl = pre.dl;
+      if (cb + 1 < BN / 64) fetch(p, t, at, row0, n0 + 32, pre);
       float v[32], dg = 0.f;
       tmem_ld32(tm + c, v);
 #pragma unroll
@@ -123,27 +129,35 @@ struct EpiUpdate {
     int tall, short_side, two;
     float a;
   };
+  struct Pre { uint4 xs[8], raw[4]; float bl; };  // 32 columns of X and its float16 copy (rows are padded to 8), diag(B)
+  static __device__ __forceinline__ void fetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int n0, Pre& pre) {
+    const int lane = threadIdx.x & 31;
+    const int64_t off = at.batch * p.stride + (int64_t)row0 * p.ld + n0;
+    fetch_piece<float, 8>(pre.xs, p.x + off, p.ld, t.M - row0, t.N - n0);
+    if (!p.two) fetch_piece<__half, 4>(pre.raw, p.xh + off, p.ld, t.M - row0, t.N - n0);
+    pre.bl = p.tall && n0 + lane < t.N ? p.bdiag[at.batch * (int64_t)p.short_side + n0 + lane] : 0.f;
+  }
+  static __device__ __forceinline__ void prefetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int half, Pre& pre) {
+    fetch(p, t, at, row0, at.n * BN + half * (BN / 2), pre);
+  }
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
-                                             uint4* stage) {
+                                             uint4* stage, Pre& pre) {
     const int row = row0 + (threadIdx.x & 31);
-    const float* bd = p.bdiag + at.batch * (int64_t)p.short_side;
-    const float bi = !p.tall && row < t.M ? bd[row] : 0.f;
+    const float bi = !p.tall && row < t.M ? p.bdiag[at.batch * (int64_t)p.short_side + row] : 0.f;
     const int64_t base = at.batch * p.stride;
 #pragma unroll 1
     for (int cb = 0; cb < BN / 64; ++cb) {
       const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c;
       if (n0 >= t.N) break;
-      const int64_t off = base + (int64_t)row * p.ld + n0;
-      float4 xs[8];
-      uint4 raw[4];
+      uint4 xs[8], raw[4];
+      turn_piece<8>(stage, pre.xs);
+      if (!p.two) turn_piece<4>(stage, pre.raw);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {  // rows are padded to 8
-        const bool in = row < t.M && n0 + 8 * q < t.N;
-        xs[2 * q] = in ? *reinterpret_cast<const float4*>(p.x + off + 8 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
-        xs[2 * q + 1] = in ? *reinterpret_cast<const float4*>(p.x + off + 8 * q + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        raw[q] = in && !p.two ? *reinterpret_cast<const uint4*>(p.xh + off + 8 * q) : make_uint4(0, 0, 0, 0);
-      }
-      const float bl = p.tall && n0 + (int)(threadIdx.x & 31) < t.N ? bd[n0 + (threadIdx.x & 31)] : 0.f;
+      for (int q = 0; q < 8; ++q) xs[q] = pre.xs[q];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) raw[q] = p.two ? make_uint4(0, 0, 0, 0) : pre.raw[q];
+      const float bl = pre.bl;
+      if (cb + 1 < BN / 64) fetch(p, t, at, row0, n0 + 32, pre);
       float v[32];
       tmem_ld32(tm + c, v);
 #pragma unroll
@@ -225,6 +239,220 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const T* __restrict__ g, i
   }
 }
 
+// ---- small matrices: short side up to 128, long side up to 256 -------------------------------------------------------
+// One CTA runs the whole iteration of a matrix and nothing leaves the SM: X (high and low float16 parts, [short][long] in
+// chunks of 64 columns, 128 swizzled bytes a row) is the operand of both products, K-major in X X^T and MN-major in B X, so the
+// same bytes serve both; A and B share one 128 x 128 buffer.  A thread holds one row and half of the columns of every
+// accumulator; A stays in its registers in fp32 until B is formed.  X is kept as high + low part (22 bits), which for a
+// bfloat16 result is as good as fp32.  What bounds it is the chain of 15 products with an epilogue and two block barriers
+// between each: 24 matrices of 128 x 128 took 183 us as 17 launches.
+constexpr int kSmallThreads = 256, kSmallChunk = 128 * 128;  // bytes of 128 rows x 64 columns
+
+__device__ __forceinline__ uint32_t small_at(int row, int col) {  // byte offset of an element in a chunked, swizzled plane
+  return (uint32_t)((col >> 6) * kSmallChunk + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4) + (col & 7) * 2);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSmallThreads)
+    ns_small_kernel(const T* __restrict__ g, int m, int n, int steps, float ca, float cb, float cc, double eps, __nv_bfloat16* __restrict__ out) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ double part[8];
+  __shared__ float diag[128];
+  __shared__ uint64_t bar_store;
+  __shared__ uint32_t tmem_slot;
+  const bool tall = m > n;
+  const int r = tall ? n : m, len = tall ? m : n, chunks = (len + 63) / 64, count = m * n;
+  const int kr = (r + 15) / 16, kl = (len + 15) / 16;  // 16-wide blocks of the two axes
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const sm = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t plane = (uint32_t)chunks * kSmallChunk;
+  uint8_t *const xh = sm, *const xl = sm + plane, *const rb = sm + 2 * plane;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, half = warp >> 2, row = q * 32 + lane;
+  const uint32_t bar = smem_u32(&bar_store), cols = len <= 128 ? 256u : 512u;
+  const T* src = g + blockIdx.x * (int64_t)count;
+  int* const err = &error_word;
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += kSmallThreads) {
+    const double v = (double)widen(src[i]);
+    s += v * v;
+  }
+  for (uint32_t i = threadIdx.x; i < (2 * plane + 2 * kSmallChunk) / 16; i += kSmallThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) part[warp] = s;
+  __syncthreads();
+  s = 0.0;
+  for (int i = 0; i < 8; ++i) s += part[i];
+  const double scale = 1.0 / (sqrt(s) + eps);
+  for (int i = threadIdx.x; i < count; i += kSmallThreads) {
+    const int gr = i / n, gc = i - gr * n;
+    const uint32_t at = tall ? small_at(gc, gr) : small_at(gr, gc);
+    const float v = (float)((double)widen(src[i]) * scale) * kXScale;
+    const __half h = __float2half_rn(v);
+    *reinterpret_cast<__half*>(xh + at) = h;
+    *reinterpret_cast<__half*>(xl + at) = __float2half_rn(v - __half2float(h));
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot, t_gram = tmem, t_upd = tmem + 128, lanes = (uint32_t)(q * 32) << 16;
+  const uint32_t a_xh = base, a_xl = base + plane, a_rb = base + 2 * plane;
+  uint32_t phase = 0;
+  bool ok = true;
+  // Everyone waits for the products issued last; all leave together when the wait ran out.
+  auto done = [&]() {
+    ok = mbar_wait(bar, phase, err, 21);
+    phase ^= 1;
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    return __syncthreads_and(ok) != 0;
+  };
+  // What the epilogue wrote to shared memory is visible to the next products.
+  auto publish = [&]() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  };
+  // 32 columns of this thread's row of a plane, from column c0 (a multiple of 32)
+  auto put32 = [&](uint8_t* p, int c0, const float (&v)[32]) {
+    uint4 o[4];
+    pack32<__half>(v, o);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(p + small_at(row, c0 + 8 * k)) = o[k];
+  };
+  const uint32_t id_sq = idesc16(false, false, false, 16 * kr, BM), id_up = idesc16(false, false, true, 16 * kl, BM);
+
+  for (int step = 0; step < steps; ++step) {
+    if (threadIdx.x == 0) {  // A: low . high, high . low, high . high
+      for (int p = 0; p < 3; ++p)
+        for (int k = 0; k < kl; ++k) {
+          const uint32_t off = (uint32_t)(k >> 2) * kSmallChunk + (k & 3) * 32;
+          mma16<false>(t_gram, desc16((p == 0 ? a_xl : a_xh) + off, false), desc16((p == 1 ? a_xl : a_xh) + off, false), id_sq, p + k > 0 ? 1u : 0u);
+        }
+      umma_commit(bar);
+    }
+    if (!done()) break;
+    float a0[32], a1[32];  // this thread's 64 columns of A
+    tmem_ld32(t_gram + lanes + half * 64, a0);
+    tmem_ld32(t_gram + lanes + half * 64 + 32, a1);
+    const int c0 = half * 64;
+    auto strip = [&](float (&v)[32], int base_col, float k, float& d) {  // takes the diagonal out
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        v[j] = (base_col + j < r && row < r) ? v[j] * k : 0.f;
+        const bool on = row == base_col + j;
+        d = on ? v[j] : d;
+        v[j] = on ? 0.f : v[j];
+      }
+    };
+    float dg = 0.f;
+    strip(a0, c0, 1.f / kXScale, dg);  // 2^12 A
+    strip(a1, c0 + 32, 1.f / kXScale, dg);
+    put32(rb, c0, a0);
+    put32(rb, c0 + 32, a1);
+    const bool mine = row >= c0 && row < c0 + 64;
+    if (mine) diag[row] = dg * (1.f / kXScale);
+    publish();
+    if (threadIdx.x == 0) {  // R R
+      for (int k = 0; k < kr; ++k) {
+        const uint32_t off = (uint32_t)(k >> 2) * kSmallChunk + (k & 3) * 32;
+        mma16<false>(t_gram, desc16(a_rb + off, false), desc16(a_rb + off, false), id_sq, k > 0 ? 1u : 0u);
+      }
+      umma_commit(bar);
+    }
+    if (!done()) break;
+    const float di = diag[row];
+    float bd = 0.f;
+    auto poly = [&](float (&rv)[32], int base_col) {
+      float v[32];
+      tmem_ld32(t_gram + lanes + base_col, v);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const int col = base_col + j;
+        const float aa = v[j] * (1.f / (kXScale * kXScale)), rij = rv[j] * (1.f / kXScale), dj = diag[col];
+        const bool on = row == col, in = col < r && row < r;
+        bd = on ? cb * di + cc * (di * di + aa) : bd;
+        rv[j] = on || !in ? 0.f : (cb * rij + cc * ((di + dj) * rij + aa)) * kBScale;
+      }
+    };
+    poly(a0, c0);
+    poly(a1, c0 + 32);
+    __syncthreads();  // R and the diagonal of A have been read
+    put32(rb, c0, a0);
+    put32(rb, c0 + 32, a1);
+    if (mine) diag[row] = bd;
+    publish();
+    if (threadIdx.x == 0) {  // B X: low part, high part
+      for (int p = 0; p < 2; ++p)
+        for (int k = 0; k < kr; ++k)
+          mma16<false>(t_upd, desc16(a_rb + (uint32_t)(k >> 2) * kSmallChunk + (k & 3) * 32, false),
+                       desc16((p == 0 ? a_xl : a_xh) + (uint32_t)k * 2048, true, kSmallChunk), id_up, p + k > 0 ? 1u : 0u);
+      umma_commit(bar);
+    }
+    if (!done()) break;
+    const float bi = diag[row];
+    const bool last = step + 1 == steps;
+    for (int c = half * 32; c < 16 * kl; c += 64) {
+      float v[32];
+      tmem_ld32(t_upd + lanes + c, v);  // columns past 16 * kl hold nothing and are not stored
+      uint4 h4[4], l4[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        h4[k] = *reinterpret_cast<const uint4*>(xh + small_at(row, c + 8 * k));
+        l4[k] = *reinterpret_cast<const uint4*>(xl + small_at(row, c + 8 * k));
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float x = __half2float(reinterpret_cast<const __half*>(h4)[j]) + __half2float(reinterpret_cast<const __half*>(l4)[j]);
+        const float y = (ca + bi) * x + v[j] * (1.f / kBScale);  // 2^12 X
+        v[j] = row < r && c + j < len ? y : 0.f;
+      }
+      if (last) {
+        uint4 o[4];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= 1.f / kXScale;
+        pack32<__nv_bfloat16>(v, o);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(xh + small_at(row, c + 8 * k)) = o[k];
+      } else {
+        put32(xh, c, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
+        put32(xl, c, v);
+      }
+    }
+    publish();
+  }
+  if (__syncthreads_and(ok)) {
+    __nv_bfloat16* dst = out + blockIdx.x * (int64_t)count;
+    for (int i = threadIdx.x; i < count; i += kSmallThreads) {
+      const int gr = i / n, gc = i - gr * n;
+      dst[i] = *reinterpret_cast<const __nv_bfloat16*>(xh + (tall ? small_at(gc, gr) : small_at(gr, gc)));
+    }
+  }
+  __syncthreads();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+
+template <typename T>
+void run_small(const Tensor& g, int64_t steps, double a, double b, double c, double eps, Tensor& out, cudaStream_t st) {
+  const int m = (int)g.size(1), n = (int)g.size(2), len = std::max(m, n);
+  const int smem = 1024 + (2 * ((len + 63) / 64) + 2) * kSmallChunk;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(ns_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  ns_small_kernel<T><<<(unsigned)g.size(0), kSmallThreads, smem, st>>>((const T*)g.data_ptr(), m, n, (int)steps, (float)a, (float)b, (float)c,
+                                                                       eps, (__nv_bfloat16*)out.data_ptr());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
 // Adds a segment: planes za, zb of batch-many matrices each.
 void add_segment(Tiles& t, int a, bool a_mn, int b, bool b_mn, int64_t K, int n, int za = 0, int zb = 0) {
   Seg& s = t.seg[t.n_seg++];
@@ -254,6 +482,12 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
   const int64_t batch = g.size(0), m = g.size(1), n = g.size(2);
   Tensor out = at::empty({batch, m, n}, g.options().dtype(at::kBFloat16));
   if (out.numel() == 0) return out;
+  if (std::min(m, n) <= 128 && std::max(m, n) <= 256 && batch < (1ll << 31)) {
+    if (g.scalar_type() == at::kFloat) run_small<float>(g, steps, a, b, c, eps, out, st);
+    else if (g.scalar_type() == at::kHalf) run_small<__half>(g, steps, a, b, c, eps, out, st);
+    else run_small<__nv_bfloat16>(g, steps, a, b, c, eps, out, st);
+    return out;
+  }
   TORCH_CHECK(batch <= 65535 && m < (1 << 30) && n < (1 << 30), "newton_schulz: sizes out of range");
   const bool tall = m > n;
   const int64_t r = std::min(m, n), ld = (n + 7) / 8 * 8, rld = (r + 7) / 8 * 8;
@@ -279,10 +513,9 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
   float *ad = diag.data_ptr<float>(), *bd = ad + batch * r;
   auto stored_x = [&](int which) { return Stored{xh0 + which * planes * plane, n, m, ld, planes * batch, m * ld}; };
   const Stored sr{rp, r, r, rld, batch, r * rld}, sb{bp, r, r, rld, batch, r * rld};
-  // columns of a tile: 256 where that still gives every pair of CTAs a tile
-  auto wide = [&](int64_t rows, int64_t tiles) { return use_pair(rows) && tiles >= sm_count() / 2; };
-  const int64_t rt = (r + 255) / 256;
-  const int bn = wide(m, batch * ((m + 255) / 256) * ((n + 255) / 256)) ? 256 : 128, sbn = wide(r, batch * (rt * (rt + 1) / 2)) ? 256 : 128;
+  const int64_t rt = (r + 255) / 256, mt = batch * ((m + 255) / 256), low = batch * (rt * (rt + 1) / 2);
+  const int bn = use_pair(m) ? pick_bn(mt * ((n + 255) / 256), mt * ((n + 127) / 128)) : 128;
+  const int sbn = use_pair(r) ? pick_bn(low, 2 * low) : 128;
   for (int64_t i = 0; i < steps; ++i) {
     const int cur = (int)(i & 1);
     {

@@ -300,6 +300,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
   int* const err = &error_word;
 
+  // The next kernel of the chain may start on idle SMs and set itself up; it waits below until this one is done.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0 && lane < maps.n) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.m[lane]) : "memory");
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
@@ -322,6 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing above reads or writes global memory
 
   // The segment is copied out of the parameters once: the compiler may not keep what it read there over an asm statement that
   // clobbers memory, and both loops below would wait for constant loads before every instruction (43 % of the tensor pipe).
@@ -520,9 +523,9 @@ inline int sm_count() {
 inline bool use_pair(int64_t M) { return M > BM; }
 
 // In a pair every CTA holds half of the tile of B, so n / 2 of each segment has to be a multiple of 64.
-inline void set_tiles(Tiles& t, int64_t M, int64_t N, int bn, int64_t batches, int splits, bool lower = false, bool pair_ok = true) {
+inline void set_tiles(Tiles& t, int64_t M, int64_t N, int bn, int64_t batches, int splits, bool lower = false, bool pair = true) {
   t.M = (int)M; t.N = (int)N; t.bn = bn;
-  t.bm = pair_ok && use_pair(M) ? 2 * BM : BM;
+  t.bm = pair && use_pair(M) ? 2 * BM : BM;
   t.mt = (int)((M + t.bm - 1) / t.bm); t.nt = (int)((N + bn - 1) / bn);
   t.batches = (int)batches; t.splits = splits; t.lower = lower ? t.bm / bn : 0;
   TORCH_CHECK(!lower || (t.lower >= 1 && t.bm % bn == 0), "dense: symmetric tiles do not fit");
@@ -530,6 +533,31 @@ inline void set_tiles(Tiles& t, int64_t M, int64_t N, int bn, int64_t batches, i
   TORCH_CHECK(per * batches * splits < (1ll << 31), "dense: too many tiles");
   t.total = (int)(per * batches * splits);
 }
+
+// The tile of a product with an epilogue of about 1 us per 64 columns (one that reads and writes several arrays), chosen by an
+// estimate of its time: rounds of tiles over the GPU, each the longer of its products (0.42 us per 64-wide block of the
+// contraction axis for 256 columns, 0.33 for 128, 0.30 for 64; measured) and its epilogue, and the last epilogue on top.  A
+// symmetric output may compute the tiles below the diagonal alone and write them twice (an epilogue 1.6 times as long).
+struct TileShape { int bn; bool pair, lower; };
+inline TileShape pick_tile(int64_t M, int64_t N, int64_t K, int64_t batches, bool symmetric) {
+  TileShape best{128, false, false};
+  double least = 1e30;
+  const double nk = (double)((K + BK - 1) / BK);
+  for (int i = 0; i < 8; ++i) {
+    const int bn = (i & 3) == 0 ? 256 : (i & 3) == 3 ? 64 : 128;
+    const bool pair = (i & 3) < 2, lower = i >= 4;
+    if ((pair && !use_pair(M)) || (lower && !symmetric)) continue;
+    Tiles t{};
+    set_tiles(t, M, N, bn, batches, 1, lower, pair);
+    const int64_t at_once = pair ? sm_count() / 2 : sm_count();
+    const double rounds = (double)((t.total + at_once - 1) / at_once), products = nk * (bn == 256 ? 0.42 : bn == 128 ? 0.33 : 0.30),
+                 epilogue = (lower ? 1.6 : 1.0) * bn / 64;
+    const double cost = rounds * std::max(products, epilogue) + std::min(products, epilogue) + (pair ? 1.0 : 0.4);
+    if (cost < least) { least = cost; best = {bn, pair, lower}; }
+  }
+  return best;
+}
+
 // Columns of a pair's tile, 256 or 128, by the number of tiles of each kind: the wide one takes less shared-memory traffic per
 // product (320 ns against 2 x 225 ns per 64-wide block), the narrow one may fill the last round of the GPU better.
 inline int pick_bn(int64_t tiles256, int64_t tiles128) {
@@ -553,16 +581,20 @@ void launch_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cu
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = PAIR ? 1 : 0;
+  cfg.numAttrs = PAIR ? 2 : 1;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, dense_kernel<BN, PAIR, Epi>, maps, t, ep));
 }
 template <int BN, typename Epi, bool PAIR_OK = true>
 void run_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cudaStream_t st) {
-  if (t.bm == BM) {
+  if constexpr (BN == 64) {
+    launch_dense<BN, false, Epi>(maps, t, ep, st);
+  } else if (t.bm == BM) {
     if constexpr (BN == 256 && !Epi::kLate) {
       TORCH_CHECK(false, "dense: 256-column tiles are for pairs");
     } else {

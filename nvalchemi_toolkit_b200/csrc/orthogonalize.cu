@@ -7,15 +7,16 @@
 // spectral norm (at most about 1.2), so float16 with a power-of-two scale (X and A times 2^12, B times 2^11) keeps 11 bits of
 // every entry that matters, three more than bfloat16.  Two choices keep its rounding from being amplified by the iteration,
 // which multiplies small singular values by up to a each step:
-//   * X itself is kept in fp32 beside its float16 copy and a X is added from there; the rounding of the copy only enters
-//     through B X and A, where it is multiplied by the row and column spaces of X and cannot feed empty directions;
+//   * X itself is kept as a float16 value and a float16 remainder (22 bits) and a X is added from both; the products read the
+//     first alone, so its rounding only enters through B X and A, where it is multiplied by the row and column spaces of X and
+//     cannot feed empty directions;
 //   * the diagonals of A and B are kept in fp32 and only the rest is rounded: A = D + R, A A = D D + D R + R D + R R, and
 //     B X = diag(B) X + (B - diag(B)) X with both terms taken from the same float16 X, so that directions in which they
 //     cancel stay empty.
 // Error of the result before its rounding: 2e-4 to 1.4e-3 of its norm over Gaussian, noisy low-rank and low-rank matrices
 // from 128 x 128 to 1024 x 1024 (bfloat16 operands: 0.4 to 2.3e-2); the rounding itself is 1.7e-3.  In matrices with a side of
-// 128 or less fewer roundings average out (up to 3e-3 at 8 x 8), while the products cost little: there X is two float16
-// values, high and low part, in A (three products) and in B X (two), which brings the error under 1e-3.
+// 128 or less fewer roundings average out (up to 3e-3 at 8 x 8), while the products cost little: there the remainder takes part
+// in A (three products) and in B X (two), which brings the error under 1e-3.
 //
 // A and B are symmetric: only tiles on and below the diagonal are computed, each is written twice.
 #include "dense16.cuh"
@@ -121,20 +122,19 @@ struct EpiUpdate {
   static constexpr int kAcc = 1, kStride = BN;
   static constexpr bool kLate = false;
   struct Params {
-    const float* x; const __half* xh; const float* bdiag;  // xh: high parts; low parts `plane` further (two != 0)
-    float* x_out; __half* xh_out; __nv_bfloat16* out;  // out != null: last step
-    int64_t ld, stride;                                // of x, xh, x_out, xh_out
+    const __half* x; const float* bdiag;   // X: high parts, remainders `plane` further
+    __half* x_out; __nv_bfloat16* out;     // out != null: last step
+    int64_t ld, stride, plane;             // of x and x_out
     int64_t out_stride;
-    int64_t plane;
-    int tall, short_side, two;
+    int tall, short_side, two;             // two: the products read the remainders as well
     float a;
   };
-  struct Pre { uint4 xs[8], raw[4]; float bl; };  // 32 columns of X and its float16 copy (rows are padded to 8), diag(B)
+  struct Pre { uint4 h[4], l[4]; float bl; };  // 32 columns of X (rows are padded to 8), diag(B)
   static __device__ __forceinline__ void fetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int n0, Pre& pre) {
     const int lane = threadIdx.x & 31;
     const int64_t off = at.batch * p.stride + (int64_t)row0 * p.ld + n0;
-    fetch_piece<float, 8>(pre.xs, p.x + off, p.ld, t.M - row0, t.N - n0);
-    if (!p.two) fetch_piece<__half, 4>(pre.raw, p.xh + off, p.ld, t.M - row0, t.N - n0);
+    fetch_piece<__half, 4>(pre.h, p.x + off, p.ld, t.M - row0, t.N - n0);
+    fetch_piece<__half, 4>(pre.l, p.x + p.plane + off, p.ld, t.M - row0, t.N - n0);
     pre.bl = p.tall && n0 + lane < t.N ? p.bdiag[at.batch * (int64_t)p.short_side + n0 + lane] : 0.f;
   }
   static __device__ __forceinline__ void prefetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int half, Pre& pre) {
@@ -144,64 +144,74 @@ struct EpiUpdate {
                                              uint4* stage, Pre& pre) {
     const int row = row0 + (threadIdx.x & 31);
     const float bi = !p.tall && row < t.M ? p.bdiag[at.batch * (int64_t)p.short_side + row] : 0.f;
+    const float two = p.two ? 1.f : 0.f;
     const int64_t base = at.batch * p.stride;
 #pragma unroll 1
     for (int cb = 0; cb < BN / 64; ++cb) {
       const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c;
       if (n0 >= t.N) break;
-      uint4 xs[8], raw[4];
-      turn_piece<8>(stage, pre.xs);
-      if (!p.two) turn_piece<4>(stage, pre.raw);
+      uint4 h4[4], l4[4];
+      turn_piece<4>(stage, pre.h);
+      turn_piece<4>(stage, pre.l);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) xs[q] = pre.xs[q];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) raw[q] = p.two ? make_uint4(0, 0, 0, 0) : pre.raw[q];
+      for (int q = 0; q < 4; ++q) { h4[q] = pre.h[q]; l4[q] = pre.l[q]; }
       const float bl = pre.bl;
       if (cb + 1 < BN / 64) fetch(p, t, at, row0, n0 + 32, pre);
       float v[32];
       tmem_ld32(tm + c, v);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float x = reinterpret_cast<const float*>(xs)[j];
+      for (int j = 0; j < 32; ++j) {  // 2^12 X
+        const float h = __half2float(reinterpret_cast<const __half*>(h4)[j]), l = __half2float(reinterpret_cast<const __half*>(l4)[j]);
         const float b = p.tall ? __shfl_sync(0xffffffffu, bl, j) : bi;
-        const float xb = p.two ? x : __half2float(reinterpret_cast<const __half*>(raw)[j]) * (1.f / kXScale);  // what the product read
-        v[j] = p.a * x + b * xb + v[j] * (1.f / (kXScale * kBScale));
+        v[j] = p.a * (h + l) + b * (h + two * l) + v[j] * (1.f / kBScale);  // b times the X that the product read
       }
       if (p.out != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= 1.f / kXScale;
         uint4 o[4];
         pack32<__nv_bfloat16>(v, o);
         __nv_bfloat16* dst = p.out + at.batch * p.out_stride;
         store_piece<__nv_bfloat16, 4>(stage, o, dst + (int64_t)row0 * t.N + n0, t.N, t.M - row0, t.N - n0,
                                       t.N % 8 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0);
       } else {
-        uint4 o[8];
-        pack32<float>(v, o);
-        store_piece<float, 8>(stage, o, p.x_out + base + (int64_t)row0 * p.ld + n0, p.ld, t.M - row0, t.N - n0, true);
+        uint4 o[4];
+        pack32<__half>(v, o);
+        __half* dst = p.x_out + base + (int64_t)row0 * p.ld + n0;
+        store_piece<__half, 4>(stage, o, dst, p.ld, t.M - row0, t.N - n0, true);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] *= kXScale;
-        uint4 oh[4];
-        pack32<__half>(v, oh);
-        __half* dst = p.xh_out + base + (int64_t)row0 * p.ld + n0;
-        store_piece<__half, 4>(stage, oh, dst, p.ld, t.M - row0, t.N - n0, true);
-        if (p.two) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
-          pack32<__half>(v, oh);
-          store_piece<__half, 4>(stage, oh, dst + p.plane, p.ld, t.M - row0, t.N - n0, true);
-        }
+        for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
+        pack32<__half>(v, o);
+        store_piece<__half, 4>(stage, o, dst + p.plane, p.ld, t.M - row0, t.N - n0, true);
       }
     }
   }
 };
 
+// Eight elements at a time where G's rows allow 16-byte accesses (8 | n, aligned), else one by one.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, int left, double (&v)[8]) {
+  if (vec) {
+    uint4 raw[sizeof(T) / 2];
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k) raw[k] = reinterpret_cast<const uint4*>(p)[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = (double)widen(reinterpret_cast<const T*>(raw)[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < left ? (double)widen(p[k]) : 0.0;
+  }
+}
+
 // Sums of squares of G in float64 (no gradient is too small or too large for them): one partial per block.
 template <typename T>
-__global__ void __launch_bounds__(256) ns_norm_kernel(const T* __restrict__ g, int64_t count, double* __restrict__ partial) {
+__global__ void __launch_bounds__(256) ns_norm_kernel(const T* __restrict__ g, int64_t count, bool vec, double* __restrict__ partial) {
   const T* src = g + blockIdx.y * count;
   double s = 0.0;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x) {
-    const double v = (double)widen(src[i]);
-    s += v * v;
+  for (int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) * 8; i < count; i += (int64_t)gridDim.x * blockDim.x * 8) {
+    double v[8];
+    load8(src + i, vec, (int)min((int64_t)8, count - i), v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += v[k] * v[k];
   }
   __shared__ double part[8];
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -213,29 +223,40 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const T* __restrict__ g, i
   }
 }
 
-// X = G / (|G| + eps) in fp32 and float16, rows padded to a multiple of 8.
+// X = G / (|G| + eps) as float16 values and remainders, times 2^12, rows padded to a multiple of 8.
 template <typename T>
-__global__ void __launch_bounds__(256) ns_init_kernel(const T* __restrict__ g, int rows, int cols, int64_t ld, const double* __restrict__ partial,
-                                                      int parts, double eps, float* __restrict__ x, __half* __restrict__ xh,
+__global__ void __launch_bounds__(256) ns_init_kernel(const T* __restrict__ g, int rows, int cols, int ld, bool vec,
+                                                      const double* __restrict__ partial, int parts, double eps, __half* __restrict__ x,
                                                       int64_t plane) {
   __shared__ double scale;
   if (threadIdx.x < 32) {
     double s = 0.0;
     for (int i = threadIdx.x; i < parts; i += 32) s += partial[blockIdx.y * parts + i];
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) scale = 1.0 / (sqrt(s) + eps);
+    if (threadIdx.x == 0) scale = (double)kXScale / (sqrt(s) + eps);
   }
   __syncthreads();
   const double k = scale;
   const T* src = g + blockIdx.y * (int64_t)rows * cols;
-  const int64_t base = blockIdx.y * (int64_t)rows * ld;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < (int64_t)rows * cols; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / cols, c = i - r * cols;
-    const float v = (float)((double)widen(src[i]) * k);
-    x[base + r * ld + c] = v;
-    const __half h = __float2half_rn(v * kXScale);
-    xh[base + r * ld + c] = h;
-    if (plane != 0) xh[plane + base + r * ld + c] = __float2half_rn(v * kXScale - __half2float(h));
+  __half* dst = x + blockIdx.y * (int64_t)rows * ld;
+  const uint32_t groups = (uint32_t)ld / 8;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < (int64_t)rows * groups; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / groups;
+    const int c = (int)(i - r * groups) * 8;
+    double v[8];
+    load8(src + r * cols + c, vec, cols - c, v);
+    float f[8];
+    uint4 h, l;
+    __half* const hp = reinterpret_cast<__half*>(&h);
+    __half* const lp = reinterpret_cast<__half*>(&l);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[j] = (float)(v[j] * k);
+      hp[j] = __float2half_rn(f[j]);
+      lp[j] = __float2half_rn(f[j] - __half2float(hp[j]));
+    }
+    *reinterpret_cast<uint4*>(dst + r * ld + c) = h;
+    *reinterpret_cast<uint4*>(dst + plane + r * ld + c) = l;
   }
 }
 
@@ -491,68 +512,71 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
   TORCH_CHECK(batch <= 65535 && m < (1 << 30) && n < (1 << 30), "newton_schulz: sizes out of range");
   const bool tall = m > n;
   const int64_t r = std::min(m, n), ld = (n + 7) / 8 * 8, rld = (r + 7) / 8 * 8;
-  const int planes = r <= 128 ? 2 : 1;
+  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>({(m * n + 4095) / 4096, 1024, std::max<int64_t>(1, 8 * sm_count() / batch)}));
+  const bool two = r <= 128;
   const int64_t plane = batch * m * ld;
   auto opt = [&](at::ScalarType t) { return g.options().dtype(t); };
-  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>({(m * n + 2047) / 2048, 1024, std::max<int64_t>(1, 4 * sm_count() / batch)}));
   Tensor partial = at::empty({batch, parts}, opt(at::kDouble));
-  Tensor x = at::empty({batch, m, ld}, opt(at::kFloat)), xh = at::empty({2, planes, batch, m, ld}, opt(at::kHalf));
+  Tensor x = at::empty({2, 2, batch, m, ld}, opt(at::kHalf));  // two iterates of [high, remainder]
   Tensor ra = at::empty({2, batch, r, rld}, opt(at::kHalf)), diag = at::empty({2, batch, r}, opt(at::kFloat));
+  __half *x0 = (__half*)x.data_ptr(), *rp = (__half*)ra.data_ptr(), *bp = rp + batch * r * rld;
+  float *ad = diag.data_ptr<float>(), *bd = ad + batch * r;
   auto prep = [&](auto v) {
     using T = decltype(v);
     const T* p = (const T*)g.data_ptr();
-    ns_norm_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(p, m * n, partial.data_ptr<double>());
-    ns_init_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(p, (int)m, (int)n, ld, partial.data_ptr<double>(), parts, eps, x.data_ptr<float>(),
-                                                          (__half*)xh.data_ptr(), planes == 2 ? plane : 0);
+    const bool vec = n % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+    ns_norm_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(p, m * n, vec, partial.data_ptr<double>());
+    ns_init_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(p, (int)m, (int)n, (int)ld, vec, partial.data_ptr<double>(), parts, eps, x0, plane);
   };
   if (g.scalar_type() == at::kFloat) prep(float{});
   else if (g.scalar_type() == at::kHalf) prep(__half{});
   else prep(__nv_bfloat16{});
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  __half *xh0 = (__half*)xh.data_ptr(), *rp = (__half*)ra.data_ptr(), *bp = rp + batch * r * rld;
-  float *ad = diag.data_ptr<float>(), *bd = ad + batch * r;
-  auto stored_x = [&](int which) { return Stored{xh0 + which * planes * plane, n, m, ld, planes * batch, m * ld}; };
+  auto stored_x = [&](int which) { return Stored{x0 + which * 2 * plane, n, m, ld, 2 * batch, m * ld}; };
   const Stored sr{rp, r, r, rld, batch, r * rld}, sb{bp, r, r, rld, batch, r * rld};
-  const int64_t rt = (r + 255) / 256, mt = batch * ((m + 255) / 256), low = batch * (rt * (rt + 1) / 2);
-  const int bn = use_pair(m) ? pick_bn(mt * ((n + 255) / 256), mt * ((n + 127) / 128)) : 128;
-  const int sbn = use_pair(r) ? pick_bn(low, 2 * low) : 128;
+  const TileShape gram = pick_tile(r, r, (two ? 3 : 1) * std::max(m, n), batch, true), poly = pick_tile(r, r, r, batch, true),
+                  upd = pick_tile(m, n, (two ? 2 : 1) * r, batch, false);
+  auto with = [](int bn, auto f) {
+    if (bn == 256) f(std::integral_constant<int, 256>{});
+    else if (bn == 128) f(std::integral_constant<int, 128>{});
+    else f(std::integral_constant<int, 64>{});
+  };
   for (int64_t i = 0; i < steps; ++i) {
     const int cur = (int)(i & 1);
-    {
+    with(gram.bn, [&](auto tag) {
+      constexpr int BN = decltype(tag)::value;
       Maps maps;
       Tiles t{};
       put_map(maps, 0, stored_x(cur));
-      for (int k = planes == 2 ? 0 : 2; k < 3; ++k)  // low . high, high . low, high . high
-        add_segment(t, 0, tall, 0, tall, tall ? m : n, sbn, k == 0 ? (int)batch : 0, k == 1 ? (int)batch : 0);
-      set_tiles(t, r, r, sbn, batch, 1, true);
-      if (sbn == 256) run_dense<256, EpiGram<256>>(maps, t, {rp, ad, rld, r * rld}, st);
-      else run_dense<128, EpiGram<128>>(maps, t, {rp, ad, rld, r * rld}, st);
-    }
-    {
+      for (int k = two ? 0 : 2; k < 3; ++k)  // remainder . high, high . remainder, high . high
+        add_segment(t, 0, tall, 0, tall, tall ? m : n, BN, k == 0 ? (int)batch : 0, k == 1 ? (int)batch : 0);
+      set_tiles(t, r, r, BN, batch, 1, gram.lower, gram.pair);
+      run_dense<BN, EpiGram<BN>>(maps, t, {rp, ad, rld, r * rld}, st);
+    });
+    with(poly.bn, [&](auto tag) {
+      constexpr int BN = decltype(tag)::value;
       Maps maps;
       Tiles t{};
       put_map(maps, 0, sr);
-      add_segment(t, 0, false, 0, false, r, sbn);
-      set_tiles(t, r, r, sbn, batch, 1, true);
-      if (sbn == 256) run_dense<256, EpiPoly<256>>(maps, t, {rp, ad, bp, bd, rld, r * rld, (float)b, (float)c}, st);
-      else run_dense<128, EpiPoly<128>>(maps, t, {rp, ad, bp, bd, rld, r * rld, (float)b, (float)c}, st);
-    }
-    Maps maps;
-    Tiles t{};
-    put_map(maps, 0, tall ? stored_x(cur) : sb);
-    put_map(maps, 1, tall ? sb : stored_x(cur));
-    for (int k = 0; k < planes; ++k) add_segment(t, 0, false, 1, !tall, r, bn, tall ? k * (int)batch : 0, tall ? 0 : k * (int)batch);
-    set_tiles(t, m, n, bn, batch, 1);
-    auto update = [&](auto tag) {
+      add_segment(t, 0, false, 0, false, r, BN);
+      set_tiles(t, r, r, BN, batch, 1, poly.lower, poly.pair);
+      run_dense<BN, EpiPoly<BN>>(maps, t, {rp, ad, bp, bd, rld, r * rld, (float)b, (float)c}, st);
+    });
+    with(upd.bn, [&](auto tag) {
       constexpr int BN = decltype(tag)::value;
-      typename EpiUpdate<BN>::Params ep{x.data_ptr<float>(), xh0 + cur * planes * plane, bd, x.data_ptr<float>(),
-                                        xh0 + (1 - cur) * planes * plane,
-                                        i + 1 == steps ? (__nv_bfloat16*)out.data_ptr() : nullptr, ld, m * ld, m * n, plane, tall ? 1 : 0, (int)r, planes - 1,
-                                        (float)a};
-      run_dense<BN, EpiUpdate<BN>>(maps, t, ep, st);
-    };
-    if (bn == 256) update(std::integral_constant<int, 256>{});
-    else update(std::integral_constant<int, 128>{});
+      Maps maps;
+      Tiles t{};
+      put_map(maps, 0, tall ? stored_x(cur) : sb);
+      put_map(maps, 1, tall ? sb : stored_x(cur));
+      for (int k = 0; k < (two ? 2 : 1); ++k)
+        add_segment(t, 0, false, 1, !tall, r, BN, tall ? k * (int)batch : 0, tall ? 0 : k * (int)batch);
+      set_tiles(t, m, n, BN, batch, 1, false, upd.pair);
+      run_dense<BN, EpiUpdate<BN>>(maps, t,
+                                   {x0 + cur * 2 * plane, bd, x0 + (1 - cur) * 2 * plane,
+                                    i + 1 == steps ? (__nv_bfloat16*)out.data_ptr() : nullptr, ld, m * ld, plane, m * n, tall ? 1 : 0, (int)r,
+                                    two ? 1 : 0, (float)a},
+                                   st);
+    });
   }
   return out;
 }

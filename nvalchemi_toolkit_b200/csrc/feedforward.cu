@@ -17,6 +17,10 @@
 
 namespace nva {
 using at::Tensor;
+
+// feedforward_rows.cu: up to 8 rows
+bool gated_ff_rows(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act, Tensor& y, cudaStream_t st);
+
 namespace {
 using namespace dense;
 
@@ -29,10 +33,18 @@ __device__ __forceinline__ void activate(float g, float& a, float& da) {
     const float s = EXACT ? 1.f / (1.f + expf(-g)) : __fdividef(1.f, 1.f + __expf(-g));
     a = g * s;
     da = s * (1.f + g * (1.f - s));
-  } else {  // g * Phi(g)
+  } else if constexpr (EXACT) {  // g * Phi(g)
     const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
     a = g * cdf;
-    da = cdf + g * 0.39894228040143268f * (EXACT ? expf(-0.5f * g * g) : __expf(-0.5f * g * g));
+    da = cdf + g * 0.39894228040143268f * expf(-0.5f * g * g);
+  } else {
+    // erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), z >= 0: Hastings' approximation (Abramowitz and Stegun,
+    // 7.1.26), off by at most 1.5e-7; its exponential is the derivative's as well
+    const float z = 0.70710678118654752f * fabsf(g), e = __expf(-0.5f * g * g), t = __fdividef(1.f, 1.f + 0.3275911f * z);
+    const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float cdf = g < 0.f ? q : 1.f - q;
+    a = g * cdf;
+    da = cdf + g * 0.39894228040143268f * e;
   }
 }
 
@@ -292,24 +304,34 @@ void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_
 
 void check_ff(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
   for (const Tensor* t : {&x, &wg, &wu, &wd})
-    TORCH_CHECK(t->is_cuda() && t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->dim() == 2,
-                "gated_ff: matrices of one type on one CUDA device");
+    TORCH_CHECK(t->is_cuda() && t->device() == x.device() && t->scalar_type() == x.scalar_type(), "gated_ff: tensors of one type on one CUDA device");
   TORCH_CHECK(x.scalar_type() == at::kFloat || x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16,
               "gated_ff: float32, float16 or bfloat16");
-  TORCH_CHECK(wg.size(0) == x.size(1) && wu.sizes() == wg.sizes() && wd.size(0) == wg.size(1), "gated_ff: shapes do not fit");
+  TORCH_CHECK(x.dim() >= 1 && wg.dim() == 2 && wu.dim() == 2 && wd.dim() == 2, "gated_ff: weights must be matrices");
+  TORCH_CHECK(wg.size(0) == x.size(-1) && wu.sizes() == wg.sizes() && wd.size(0) == wg.size(1), "gated_ff: shapes do not fit");
   TORCH_CHECK(act == kSilu || act == kGelu, "gated_ff: unknown activation");
-  TORCH_CHECK(x.size(0) < (1ll << 31) && x.size(1) >= 1 && wg.size(1) >= 1 && wd.size(1) >= 1, "gated_ff: sizes out of range");
+  TORCH_CHECK(x.size(-1) >= 1 && wg.size(1) >= 1 && wd.size(1) >= 1, "gated_ff: sizes out of range");
+  TORCH_CHECK(x.numel() / x.size(-1) < (1ll << 31) && x.size(-1) < (1ll << 31) && wg.size(1) < (1ll << 31) && wd.size(1) < (1ll << 31),
+              "gated_ff: sizes out of range");
+}
+Tensor as_matrix(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)}); }
+std::vector<int64_t> out_sizes(const Tensor& x, int64_t n) {
+  std::vector<int64_t> s = x.sizes().vec();
+  s.back() = n;
+  return s;
 }
 
 }  // namespace
 
-Tensor gated_ff_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
-  check_ff(x, wg, wu, wd, act);
-  c10::cuda::CUDAGuard guard(x.device());
+Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
+  check_ff(x_in, wg, wu, wd, act);
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = as_matrix(x_in);
   const int64_t M = x.size(0), H = wg.size(1), N = wd.size(1);
-  Tensor y = at::empty({M, N}, x.options());
+  Tensor y = at::empty(out_sizes(x_in, N), x.options());
   if (M == 0) return y;
   auto st = at::cuda::getCurrentCUDAStream();
+  if (gated_ff_rows(x, wg, wu, wd, act, y, st)) return y;
   const int P = planes_of(x);
   const bool bf16 = x.scalar_type() != at::kHalf;
   Operand ox = operand(x, st), og = operand(wg, st), ou = operand(wu, st), od = operand(wd, st);
@@ -344,15 +366,16 @@ Tensor gated_ff_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const T
 }
 
 // which: bit 0 dx, bit 1 dWg and dWu, bit 2 dWd; the others come back empty.
-std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy, const Tensor& x, const Tensor& wg, const Tensor& wu,
+std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, const Tensor& x_in, const Tensor& wg, const Tensor& wu,
                                                         const Tensor& wd, int64_t act, int64_t which) {
-  check_ff(x, wg, wu, wd, act);
-  const int64_t M = x.size(0), K = x.size(1), H = wg.size(1), N = wd.size(1);
-  TORCH_CHECK(dy.device() == x.device() && dy.scalar_type() == x.scalar_type() && dy.dim() == 2 && dy.size(0) == M && dy.size(1) == N,
+  check_ff(x_in, wg, wu, wd, act);
+  TORCH_CHECK(dy_in.device() == x_in.device() && dy_in.scalar_type() == x_in.scalar_type() && dy_in.sizes().vec() == out_sizes(x_in, wd.size(1)),
               "gated_ff: dy does not fit");
-  c10::cuda::CUDAGuard guard(x.device());
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = as_matrix(x_in), dy = as_matrix(dy_in);
+  const int64_t M = x.size(0), K = x.size(1), H = wg.size(1), N = wd.size(1);
   auto st = at::cuda::getCurrentCUDAStream();
-  Tensor dx = at::empty({which & 1 ? M : 0, K}, x.options()), dgu = at::empty({2, which & 2 ? K : 0, H}, x.options()),
+  Tensor dx = which & 1 ? at::empty(x_in.sizes(), x.options()) : at::empty({0}, x.options()), dgu = at::empty({2, which & 2 ? K : 0, H}, x.options()),
          dwd = at::empty({which & 4 ? H : 0, N}, x.options());
   if (M == 0 || (which & 7) == 0) {
     dgu.zero_();

@@ -8,8 +8,10 @@
 // registers of the threads that loaded it (TPR threads, VPT vectors of VEC elements each), so the mean and the centred
 // second moment are two exact passes over registers and nothing is read twice.  Statistics and all sums are fp32 (float64
 // rows: float64); only the stored results are rounded to the tensors' types.
-// The backward grid is persistent: a thread owns the same columns in every row it visits and keeps their dw / db sums in
-// registers; the block's row groups are added in a fixed order in shared memory, one partial row per block goes to the
+// What counts is bytes under way: 64 bytes a thread (R rows of a group at a time where rows are short) and many resident
+// threads; loading the next rows ahead of a persistent block's reductions costs registers and with them residency, and was
+// slower (16,384 x 4096 float16 backward 182 us against 112 us).  In the backward pass the grid is persistent, a thread owns the same columns in every row it visits and keeps their dw / db sums in
+// registers; a block's row groups are added in a fixed order in shared memory, one partial row per block goes to the
 // workspace, and a second kernel adds the partial rows in a fixed order, so results do not change from run to run.
 #include "common.cuh"
 
@@ -26,69 +28,103 @@ template <typename A> __device__ __forceinline__ A inv_sqrt(A x);
 template <> __device__ __forceinline__ float inv_sqrt<float>(float x) { return 1.f / sqrtf(x); }
 template <> __device__ __forceinline__ double inv_sqrt<double>(double x) { return 1.0 / sqrt(x); }
 
-// Sum over the TPR threads that share a row; every one of them gets it.  TPR > 32: the whole block is one row group.
-template <int TPR, typename A>
-__device__ __forceinline__ A row_sum(A v, A* scratch) {
+// Sums over the TPR threads that share a row; every one of them gets them.  TPR > 32: the whole block is one row group, and
+// two buffers take turns, so that one barrier per call is enough.
+template <int TPR, int N, typename A>
+__device__ __forceinline__ void row_sum(A (&v)[N], A (*scratch)[N][32], int& turn) {
 #pragma unroll
-  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
   if constexpr (TPR > 32) {
     constexpr int W = TPR / 32;
-    __syncthreads();  // the previous use of scratch has been read
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[0];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0)
 #pragma unroll
-    for (int i = 1; i < W; ++i) v += scratch[i];
+      for (int n = 0; n < N; ++n) scratch[turn][n][threadIdx.x >> 5] = v[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n] = scratch[turn][n][0];
+#pragma unroll
+      for (int i = 1; i < W; ++i) v[n] += scratch[turn][n][i];
+    }
   }
-  return v;
 }
 
 template <int TPR> constexpr int kBlock = TPR > 32 ? TPR : 256;  // threads of a block
 
-template <typename T, typename W, int VEC, int TPR, int VPT>
+// threads of a block that leave room for two more blocks of 256 on the SM
+template <int TPR> constexpr int kMinBlocks = kBlock<TPR> == 256 && TPR > 32 ? 3 : 1;
+
+template <typename T, int VEC, int TPR, int VPT>
+__device__ __forceinline__ void load_row(Pack<T, VEC> (&p)[VPT], const T* src, int64_t row, int64_t ld, int64_t rows, int cols, int lane) {
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = (i * TPR + lane) * VEC;
+    if (row < rows && c < cols) p[i] = *reinterpret_cast<const Pack<T, VEC>*>(src + row * ld + c);
+  }
+}
+
+template <typename T, typename W, int VEC, int TPR, int VPT, int R>
 __global__ void __launch_bounds__(kBlock<TPR>)
     layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b,
                           T* __restrict__ y, typename AccOf<T>::type* __restrict__ mean,
                           typename AccOf<T>::type* __restrict__ rstd, int64_t rows, int cols, double eps) {
   using A = typename AccOf<T>::type;
-  __shared__ A scratch[32];
+  __shared__ A scratch[2][R][32];
+  int turn = 0;
   constexpr int RPB = kBlock<TPR> / TPR;
   const int lane = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  const bool live = row < rows;  // dead groups take part in the shuffles with zeros
-  A v[VPT * VEC];
-  A sum = 0;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = (i * TPR + lane) * VEC;
-    if (live && c < cols) {
-      const Pack<T, VEC> p = *reinterpret_cast<const Pack<T, VEC>*>(x + row * ldx + c);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) { v[i * VEC + k] = widen(p.v[k]); sum += v[i * VEC + k]; }
-    }
-  }
+  const int64_t row0 = (int64_t)blockIdx.x * (RPB * R) + threadIdx.x / TPR;  // rows past the end take part in the sums with zeros
   const A inv_n = (A)1 / (A)cols;
-  const A mu = row_sum<TPR>(sum, scratch) * inv_n;
-  A sq = 0;
+  Pack<T, VEC> p[R][VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (live && (i * TPR + lane) * VEC < cols)
+  for (int r = 0; r < R; ++r) load_row<T, VEC, TPR, VPT>(p[r], x, row0 + r * RPB, ldx, rows, cols, lane);
+  A sum[R];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) { const A d = v[i * VEC + k] - mu; sq += d * d; }
-  const A r = inv_sqrt<A>(row_sum<TPR>(sq, scratch) * inv_n + (A)eps);
-  if (!live) return;
-  if (lane == 0 && mean != nullptr) { mean[row] = mu; rstd[row] = r; }
+  for (int r = 0; r < R; ++r) {
+    sum[r] = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (row0 + r * RPB < rows && (i * TPR + lane) * VEC < cols)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[r] += widen(p[r][i].v[k]);
+  }
+  row_sum<TPR>(sum, scratch, turn);
+  A sq[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    sum[r] *= inv_n;
+    sq[r] = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (row0 + r * RPB < rows && (i * TPR + lane) * VEC < cols)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) { const A d = widen(p[r][i].v[k]) - sum[r]; sq[r] += d * d; }
+  }
+  row_sum<TPR>(sq, scratch, turn);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t row = row0 + r * RPB;
+    sq[r] = inv_sqrt<A>(sq[r] * inv_n + (A)eps);
+    if (lane == 0 && row < rows && mean != nullptr) { mean[row] = sum[r]; rstd[row] = sq[r]; }
+  }
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = (i * TPR + lane) * VEC;
-    if (c < cols) {
-      Pack<W, VEC> pw, pb;
-      if (w != nullptr) pw = *reinterpret_cast<const Pack<W, VEC>*>(w + c);
-      if (b != nullptr) pb = *reinterpret_cast<const Pack<W, VEC>*>(b + c);
+    if (c >= cols) continue;
+    Pack<W, VEC> pw, pb;
+    if (w != nullptr) pw = *reinterpret_cast<const Pack<W, VEC>*>(w + c);
+    if (b != nullptr) pb = *reinterpret_cast<const Pack<W, VEC>*>(b + c);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * RPB;
+      if (row >= rows) continue;
       Pack<T, VEC> o;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
-        A t = (v[i * VEC + k] - mu) * r;
+        A t = (widen(p[r][i].v[k]) - sum[r]) * sq[r];
         if (w != nullptr) t *= widen(pw.v[k]);
         if (b != nullptr) t += widen(pb.v[k]);
         o.v[k] = narrow<T>(t);
@@ -99,67 +135,74 @@ __global__ void __launch_bounds__(kBlock<TPR>)
 }
 
 // partial [gridDim.x][2][cols]: this block's sums of g xh and g (null when neither gradient is wanted).
-template <typename T, typename W, int VEC, int TPR, int VPT>
-__global__ void __launch_bounds__(kBlock<TPR>)
+template <typename T, typename W, int VEC, int TPR, int VPT, int R>
+__global__ void __launch_bounds__(kBlock<TPR>, kMinBlocks<TPR>)
     layer_norm_bwd_kernel(const T* __restrict__ g, int64_t ldg, const T* __restrict__ x, int64_t ldx,
                           const typename AccOf<T>::type* __restrict__ mean, const typename AccOf<T>::type* __restrict__ rstd,
                           const W* __restrict__ w, T* __restrict__ dx, typename AccOf<T>::type* __restrict__ partial,
                           int64_t rows, int cols) {
   using A = typename AccOf<T>::type;
   constexpr int THREADS = kBlock<TPR>, RPB = THREADS / TPR, E = VPT * VEC;
-  __shared__ A scratch[32];
+  __shared__ A scratch[2][2 * R][32];
+  int turn = 0;
   __shared__ A fold[RPB > 1 ? THREADS * VEC : 1];
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   A dw[E], db[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) { dw[i] = 0; db[i] = 0; }
   const A inv_n = (A)1 / (A)cols;
-  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < rows; row0 += (int64_t)gridDim.x * RPB) {
-    const int64_t row = row0 + group;
-    const bool live = row < rows;
-    Pack<T, VEC> pg[VPT], px[VPT];
-    A mu = 0, r = 0;
-    if (live) { mu = mean[row]; r = rstd[row]; }
+  for (int64_t block0 = (int64_t)blockIdx.x * (RPB * R); block0 < rows; block0 += (int64_t)gridDim.x * (RPB * R)) {
+    const int64_t row0 = block0 + group;
+    Pack<T, VEC> pg[R][VPT], px[R][VPT];
+    A mu[R], rs[R], s[2 * R];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (live && c < cols) {
-        pg[i] = *reinterpret_cast<const Pack<T, VEC>*>(g + row * ldg + c);
-        px[i] = *reinterpret_cast<const Pack<T, VEC>*>(x + row * ldx + c);
-      }
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * RPB;
+      load_row<T, VEC, TPR, VPT>(pg[r], g, row, ldg, rows, cols, lane);
+      load_row<T, VEC, TPR, VPT>(px[r], x, row, ldx, rows, cols, lane);
+      mu[r] = row < rows ? mean[row] : (A)0;
+      rs[r] = row < rows ? rstd[row] : (A)0;
+      s[2 * r] = 0;
+      s[2 * r + 1] = 0;
     }
-    A s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = (i * TPR + lane) * VEC;
-      if (live && c < cols) {
-        Pack<W, VEC> pw;
-        if (w != nullptr) pw = *reinterpret_cast<const Pack<W, VEC>*>(w + c);
+      if (c >= cols) continue;
+      Pack<W, VEC> pw;
+      if (w != nullptr) pw = *reinterpret_cast<const Pack<W, VEC>*>(w + c);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (row0 + r * RPB >= rows) continue;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          const A gv = widen(pg[i].v[k]), xh = (widen(px[i].v[k]) - mu) * r;
+          const A gv = widen(pg[r][i].v[k]), xh = (widen(px[r][i].v[k]) - mu[r]) * rs[r];
           dw[i * VEC + k] += gv * xh;
           db[i * VEC + k] += gv;
           const A gw = w != nullptr ? gv * widen(pw.v[k]) : gv;
-          s1 += gw;
-          s2 += gw * xh;
+          s[2 * r] += gw;
+          s[2 * r + 1] += gw * xh;
         }
       }
     }
-    s1 = row_sum<TPR>(s1, scratch) * inv_n;
-    s2 = row_sum<TPR>(s2, scratch) * inv_n;
+    row_sum<TPR>(s, scratch, turn);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = (i * TPR + lane) * VEC;
-      if (live && c < cols) {
-        Pack<W, VEC> pw;
-        if (w != nullptr) pw = *reinterpret_cast<const Pack<W, VEC>*>(w + c);
+      if (c >= cols) continue;
+      Pack<W, VEC> pw;
+      if (w != nullptr) pw = *reinterpret_cast<const Pack<W, VEC>*>(w + c);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int64_t row = row0 + r * RPB;
+        if (row >= rows) continue;
+        const A s1 = s[2 * r] * inv_n, s2 = s[2 * r + 1] * inv_n;
         Pack<T, VEC> o;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          const A gv = widen(pg[i].v[k]), xh = (widen(px[i].v[k]) - mu) * r;
+          const A gv = widen(pg[r][i].v[k]), xh = (widen(px[r][i].v[k]) - mu[r]) * rs[r];
           const A gw = w != nullptr ? gv * widen(pw.v[k]) : gv;
-          o.v[k] = narrow<T>(r * (gw - s1 - xh * s2));
+          o.v[k] = narrow<T>(rs[r] * (gw - s1 - xh * s2));
         }
         *reinterpret_cast<Pack<T, VEC>*>(dx + row * cols + c) = o;
       }
@@ -193,26 +236,31 @@ __global__ void __launch_bounds__(kBlock<TPR>)
   }
 }
 
-// Column sums of partial [blocks][2 cols]: 32 columns per block, 32 threads down each of them, added in a fixed order.
-template <typename A, typename W>
+// Column sums of partial [blocks][2 cols], added in a fixed order: COLS columns per block, 1024 / COLS threads down each of
+// them.  32 columns read whole cache lines (8192 column sums of 444 rows: 5 us against 15 us), 8 columns (a 32-byte sector) give
+// narrow rows four times the blocks (256 of 592: 4 us against 7 us).
+template <typename A, typename W, int COLS>
 __global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const A* __restrict__ partial, int blocks, int cols,
                                                                W* __restrict__ dw, W* __restrict__ db) {
-  __shared__ A tile[32][33];
-  const int c = blockIdx.x * 32 + threadIdx.x;
+  constexpr int DOWN = 1024 / COLS;
+  __shared__ A tile[DOWN][COLS + 1];
+  const int x = threadIdx.x % COLS, y = threadIdx.x / COLS, c = blockIdx.x * COLS + x;
   A s = 0;
   if (c < 2 * cols)
-    for (int i = threadIdx.y; i < blocks; i += 32) s += partial[(int64_t)i * 2 * cols + c];
-  tile[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.y == 0 && c < 2 * cols) {
-    s = 0;
-    for (int i = 0; i < 32; ++i) s += tile[i][threadIdx.x];
-    if (c < cols) { if (dw != nullptr) dw[c] = narrow<W>(s); }
-    else if (db != nullptr) db[c - cols] = narrow<W>(s);
+#pragma unroll 4
+    for (int i = y; i < blocks; i += DOWN) s += partial[(int64_t)i * 2 * cols + c];
+  tile[y][x] = s;
+  for (int o = DOWN / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (y < o) tile[y][x] += tile[y + o][x];
+  }
+  if (y == 0 && c < 2 * cols) {
+    if (c < cols) { if (dw != nullptr) dw[c] = narrow<W>(tile[0][x]); }
+    else if (db != nullptr) db[c - cols] = narrow<W>(tile[0][x]);
   }
 }
 
-constexpr int64_t kMaxCols = 8192;
+constexpr int64_t kMaxCols = 8192;  // messages name it as text: the extension links its own iostreams, which cannot format numbers
 
 struct LnArgs {
   const void *g, *x, *w, *b;
@@ -224,50 +272,71 @@ struct LnArgs {
   cudaStream_t st;
 };
 
-template <typename T, typename W, int VEC, int TPR, int VPT>
-int launch(const LnArgs& a, bool count_only) {
+template <typename T, typename W, int VEC, int TPR, int VPT, int R>
+int forward(const LnArgs& a) {
   using A = typename AccOf<T>::type;
   constexpr int THREADS = kBlock<TPR>, RPB = THREADS / TPR;
-  const int64_t need = (a.rows + RPB - 1) / RPB;
-  if (!a.backward) {
-    TORCH_CHECK(need < (int64_t)2147483647, "layer_norm: too many rows");
-    layer_norm_fwd_kernel<T, W, VEC, TPR, VPT><<<(unsigned)need, THREADS, 0, a.st>>>(
-        (const T*)a.x, a.ldx, (const W*)a.w, (const W*)a.b, (T*)a.y, (A*)a.mean, (A*)a.rstd, a.rows, a.cols, a.eps);
-    return 0;
-  }
+  const int64_t blocks = (a.rows + RPB * R - 1) / (RPB * R);
+  TORCH_CHECK(blocks < (int64_t)2147483647, "layer_norm: too many rows");
+  layer_norm_fwd_kernel<T, W, VEC, TPR, VPT, R><<<(unsigned)blocks, THREADS, 0, a.st>>>(
+      (const T*)a.x, a.ldx, (const W*)a.w, (const W*)a.b, (T*)a.y, (A*)a.mean, (A*)a.rstd, a.rows, a.cols, a.eps);
+  return 0;
+}
+
+template <typename T, typename W, int VEC, int TPR, int VPT, int R>
+int backward(const LnArgs& a, bool count_only) {
+  using A = typename AccOf<T>::type;
+  constexpr int THREADS = kBlock<TPR>, RPB = THREADS / TPR;
   if (count_only) {  // blocks of the persistent grid: what fits on the GPU at once, less when there are fewer rows
     int per_sm = 1, dev = 0, sms = 148;
     C10_CUDA_CHECK(cudaGetDevice(&dev));
     C10_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, layer_norm_bwd_kernel<T, W, VEC, TPR, VPT>, THREADS, 0));
-    return (int)std::min<int64_t>(need, (int64_t)sms * std::max(per_sm, 1));
+    C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, layer_norm_bwd_kernel<T, W, VEC, TPR, VPT, R>, THREADS, 0));
+    return (int)std::min<int64_t>((a.rows + RPB * R - 1) / (RPB * R), (int64_t)sms * std::max(per_sm, 1));
   }
-  layer_norm_bwd_kernel<T, W, VEC, TPR, VPT><<<a.blocks, THREADS, 0, a.st>>>(
+  layer_norm_bwd_kernel<T, W, VEC, TPR, VPT, R><<<a.blocks, THREADS, 0, a.st>>>(
       (const T*)a.g, a.ldg, (const T*)a.x, a.ldx, (const A*)a.mean, (const A*)a.rstd, (const W*)a.w, (T*)a.y, (A*)a.partial,
       a.rows, a.cols);
   return a.blocks;
 }
 
-// Threads per row: a part of a warp for short rows (no idle lanes, no shared memory), the whole warp up to four vectors a
-// lane, a block of its own for longer rows.
+// Threads per row: a part of a warp for short rows (no idle lanes), the warp with up to four vectors a lane, then a block with
+// two or four (a warp with 16 vectors a lane needs no barrier, but 16,384 x 4096 float16 forward took 71 us against 57 us).
 template <typename T, typename W, int VEC>
 int pick(const LnArgs& a, bool count_only) {
   const int nv = (a.cols + VEC - 1) / VEC;
   if constexpr (VEC == 1) {
-    if (nv <= 128) return launch<T, W, 1, 32, 4>(a, count_only);
-    if (nv <= 512) return launch<T, W, 1, 32, 16>(a, count_only);
-    if (nv <= 2048) return launch<T, W, 1, 128, 16>(a, count_only);
-    return launch<T, W, 1, 512, 16>(a, count_only);
+    if (!a.backward) {
+      if (nv <= 128) return forward<T, W, 1, 32, 4, 2>(a);
+      if (nv <= 512) return forward<T, W, 1, 128, 4, 1>(a);
+      if (nv <= 2048) return forward<T, W, 1, 512, 4, 1>(a);
+      return forward<T, W, 1, 512, 16, 1>(a);
+    }
+    if (nv <= 128) return backward<T, W, 1, 32, 4, 1>(a, count_only);
+    if (nv <= 512) return backward<T, W, 1, 128, 4, 1>(a, count_only);
+    if (nv <= 2048) return backward<T, W, 1, 512, 4, 1>(a, count_only);
+    return backward<T, W, 1, 512, 16, 1>(a, count_only);
   } else {
-    if (nv <= 8) return launch<T, W, VEC, 8, 1>(a, count_only);
-    if (nv <= 16) return launch<T, W, VEC, 16, 1>(a, count_only);
-    if (nv <= 32) return launch<T, W, VEC, 32, 1>(a, count_only);
-    if (nv <= 64) return launch<T, W, VEC, 32, 2>(a, count_only);
-    if (nv <= 128) return launch<T, W, VEC, 32, 4>(a, count_only);
-    if (nv <= 256) return launch<T, W, VEC, 128, 2>(a, count_only);
-    if (nv <= 512) return launch<T, W, VEC, 256, 2>(a, count_only);
-    if (nv <= 1024) return launch<T, W, VEC, 512, 2>(a, count_only);
-    return launch<T, W, VEC, 512, 16 / VEC>(a, count_only);
+    if (!a.backward) {
+      if (nv <= 8) return forward<T, W, VEC, 8, 1, 4>(a);
+      if (nv <= 16) return forward<T, W, VEC, 16, 1, 4>(a);
+      if (nv <= 32) return forward<T, W, VEC, 32, 1, 4>(a);
+      if (nv <= 64) return forward<T, W, VEC, 32, 2, 2>(a);
+      if (nv <= 128) return forward<T, W, VEC, 32, 4, 1>(a);
+      if (nv <= 256) return forward<T, W, VEC, 128, 2, 1>(a);
+      if (nv <= 512) return forward<T, W, VEC, 256, 2, 1>(a);
+      if (nv <= 1024) return forward<T, W, VEC, 256, 4, 1>(a);
+      return forward<T, W, VEC, 512, 16 / VEC, 1>(a);
+    }
+    if (nv <= 8) return backward<T, W, VEC, 8, 1, 2>(a, count_only);
+    if (nv <= 16) return backward<T, W, VEC, 16, 1, 2>(a, count_only);
+    if (nv <= 32) return backward<T, W, VEC, 32, 1, 2>(a, count_only);
+    if (nv <= 64) return backward<T, W, VEC, 32, 2, 1>(a, count_only);
+    if (nv <= 128) return backward<T, W, VEC, 32, 4, 1>(a, count_only);
+    if (nv <= 256) return backward<T, W, VEC, 128, 2, 1>(a, count_only);
+    if (nv <= 512) return backward<T, W, VEC, 256, 2, 1>(a, count_only);
+    if (nv <= 1024) return backward<T, W, VEC, 512, 2, 1>(a, count_only);
+    return backward<T, W, VEC, 512, 16 / VEC, 1>(a, count_only);
   }
 }
 
@@ -282,76 +351,99 @@ int pick_vec(const LnArgs& a, bool count_only) {
   return vec ? pick<T, W, VEC>(a, count_only) : pick<T, W, 1>(a, count_only);
 }
 
+void check_types(at::ScalarType xt, at::ScalarType wt) {
+  TORCH_CHECK((xt == at::kFloat || xt == at::kDouble || xt == at::kBFloat16 || xt == at::kHalf) && (wt == xt || (wt == at::kFloat && xt != at::kDouble)),
+              "layer_norm: rows of type ", xt, " with weights of type ", wt, " are not supported");
+}
+
 int dispatch(const LnArgs& a, at::ScalarType xt, at::ScalarType wt, bool count_only) {
   if (xt == at::kFloat && wt == at::kFloat) return pick_vec<float, float>(a, count_only);
   if (xt == at::kDouble && wt == at::kDouble) return pick_vec<double, double>(a, count_only);
   if (xt == at::kBFloat16 && wt == at::kBFloat16) return pick_vec<__nv_bfloat16, __nv_bfloat16>(a, count_only);
   if (xt == at::kBFloat16 && wt == at::kFloat) return pick_vec<__nv_bfloat16, float>(a, count_only);
   if (xt == at::kHalf && wt == at::kHalf) return pick_vec<__half, __half>(a, count_only);
-  if (xt == at::kHalf && wt == at::kFloat) return pick_vec<__half, float>(a, count_only);
-  TORCH_CHECK(false, "layer_norm: rows of type ", xt, " with weights of type ", wt, " are not supported");
+  return pick_vec<__half, float>(a, count_only);  // check_types has passed
 }
 
-void check_rows(const Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (t.size(1) == 1 || t.stride(1) == 1 || t.numel() == 0), "layer_norm: ", name,
-              " must be a CUDA matrix with contiguous rows");
+// Any tensor as a matrix with contiguous rows: a view where the strides allow one.
+Tensor as_rows(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() >= 1, "layer_norm: ", name, " must be a CUDA tensor with at least one axis");
+  const int64_t cols = t.size(-1);
+  TORCH_CHECK(cols >= 1 && cols <= kMaxCols, "layer_norm: row length must lie in 1..8192");
+  Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / cols, cols});
+  return r.stride(1) == 1 || cols == 1 || r.numel() == 0 ? r : r.contiguous();
 }
-void check_vector(const c10::optional<Tensor>& t, const Tensor& x, const char* name) {
-  if (!t.has_value()) return;
-  TORCH_CHECK(t->device() == x.device() && t->dim() == 1 && t->is_contiguous() && t->size(0) == x.size(1), "layer_norm: ", name,
-              " must be a contiguous vector of the row length on the device of x");
+c10::optional<Tensor> as_vector(const c10::optional<Tensor>& t, const Tensor& x, const char* name) {
+  if (!t.has_value()) return t;
+  TORCH_CHECK(t->device() == x.device() && t->dim() == 1 && t->size(0) == x.size(-1), "layer_norm: ", name,
+              " must be a vector of the row length on the device of x");
+  return t->is_contiguous() ? *t : t->contiguous();
 }
 void* ptr(const c10::optional<Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
-}  // namespace
-
-std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x, const c10::optional<Tensor>& weight,
-                                                  const c10::optional<Tensor>& bias, double eps, bool stats) {
-  check_rows(x, "x");
-  check_vector(weight, x, "weight");
-  check_vector(bias, x, "bias");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= kMaxCols, "layer_norm: row length must lie in 1..", kMaxCols);
-  const at::ScalarType wt = weight.has_value() ? weight->scalar_type() : bias.has_value() ? bias->scalar_type() : x.scalar_type();
-  TORCH_CHECK(!bias.has_value() || bias->scalar_type() == wt, "layer_norm: weight and bias must have one type");
-  c10::cuda::CUDAGuard guard(x.device());
-  Tensor y = at::empty({x.size(0), x.size(1)}, x.options());
-  auto so = x.options().dtype(x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat);
-  Tensor mean = at::empty({stats ? x.size(0) : 0}, so), rstd = at::empty({stats ? x.size(0) : 0}, so);
-  if (x.size(0) == 0) return {y, mean, rstd};
+Tensor forward_pass(const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps, Tensor* mean,
+                    Tensor* rstd) {
+  c10::cuda::OptionalCUDAGuard guard;
+  if (x.is_cuda()) guard.set_device(x.device());
+  const Tensor rows = as_rows(x, "x");
+  const auto w = as_vector(weight, x, "weight"), b = as_vector(bias, x, "bias");
+  const at::ScalarType wt = w.has_value() ? w->scalar_type() : b.has_value() ? b->scalar_type() : x.scalar_type();
+  TORCH_CHECK(!b.has_value() || b->scalar_type() == wt, "layer_norm: weight and bias must have one type");
+  Tensor y = at::empty(x.sizes(), x.options());
+  if (mean != nullptr) {
+    auto so = x.options().dtype(x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat);
+    *mean = at::empty({rows.size(0)}, so);
+    *rstd = at::empty({rows.size(0)}, so);
+  }
   LnArgs a{};
-  a.x = x.data_ptr(); a.w = ptr(weight); a.b = ptr(bias); a.y = y.data_ptr();
-  a.mean = stats ? mean.data_ptr() : nullptr; a.rstd = stats ? rstd.data_ptr() : nullptr;
-  a.ldx = x.stride(0); a.rows = x.size(0); a.cols = (int)x.size(1); a.eps = eps;
+  a.x = rows.data_ptr(); a.w = ptr(w); a.b = ptr(b); a.y = y.data_ptr();
+  a.mean = mean != nullptr ? mean->data_ptr() : nullptr; a.rstd = mean != nullptr ? rstd->data_ptr() : nullptr;
+  a.ldx = rows.stride(0); a.rows = rows.size(0); a.cols = (int)rows.size(1); a.eps = eps;
   a.st = at::cuda::getCurrentCUDAStream();
+  check_types(x.scalar_type(), wt);
+  if (a.rows == 0) return y;
   dispatch(a, x.scalar_type(), wt, false);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return y;
+}
+
+}  // namespace
+
+Tensor layer_norm_apply(const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps) {
+  return forward_pass(x, weight, bias, eps, nullptr, nullptr);
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x, const c10::optional<Tensor>& weight,
+                                                  const c10::optional<Tensor>& bias, double eps) {
+  Tensor mean, rstd;
+  Tensor y = forward_pass(x, weight, bias, eps, &mean, &rstd);
   return {y, mean, rstd};
 }
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad, const Tensor& x, const Tensor& mean, const Tensor& rstd,
                                                   const c10::optional<Tensor>& weight, bool want_params,
                                                   c10::optional<at::ScalarType> param_type) {
-  check_rows(x, "x");
-  check_rows(grad, "grad");
-  check_vector(weight, x, "weight");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= kMaxCols, "layer_norm: row length must lie in 1..", kMaxCols);
   TORCH_CHECK(grad.sizes() == x.sizes() && grad.scalar_type() == x.scalar_type() && grad.device() == x.device(),
               "layer_norm: grad must match x");
+  c10::cuda::OptionalCUDAGuard guard;
+  if (x.is_cuda()) guard.set_device(x.device());
+  const Tensor xr = as_rows(x, "x"), gr = as_rows(grad, "grad");
+  const auto w = as_vector(weight, x, "weight");
   const at::ScalarType st = x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat;
   for (const Tensor* s : {&mean, &rstd})
-    TORCH_CHECK(s->device() == x.device() && s->dim() == 1 && s->is_contiguous() && s->size(0) == x.size(0) && s->scalar_type() == st,
+    TORCH_CHECK(s->device() == x.device() && s->dim() == 1 && s->is_contiguous() && s->size(0) == xr.size(0) && s->scalar_type() == st,
                 "layer_norm: mean and rstd must be the forward pass's statistics");
-  const at::ScalarType wt = weight.has_value() ? weight->scalar_type() : param_type.value_or(x.scalar_type());
-  c10::cuda::CUDAGuard guard(x.device());
-  const int64_t cols = x.size(1);
-  Tensor dx = at::empty({x.size(0), cols}, x.options());
-  Tensor dw = at::empty({want_params ? cols : 0}, x.options().dtype(wt)), db = at::empty_like(dw);
-  if (x.size(0) == 0) return {dx, dw.zero_(), db.zero_()};
+  const at::ScalarType wt = w.has_value() ? w->scalar_type() : param_type.value_or(x.scalar_type());
+  check_types(x.scalar_type(), wt);
+  const int64_t cols = xr.size(1);
+  Tensor dx = at::empty(x.sizes(), x.options());
+  Tensor dw = at::empty({want_params ? cols : 0}, x.options().dtype(wt)), db = at::empty({want_params ? cols : 0}, x.options().dtype(wt));
+  if (xr.size(0) == 0) return {dx, dw.zero_(), db.zero_()};
   LnArgs a{};
   a.backward = true;
-  a.g = grad.data_ptr(); a.x = x.data_ptr(); a.w = ptr(weight); a.y = dx.data_ptr();
+  a.g = gr.data_ptr(); a.x = xr.data_ptr(); a.w = ptr(w); a.y = dx.data_ptr();
   a.mean = mean.data_ptr(); a.rstd = rstd.data_ptr();
-  a.ldg = grad.stride(0); a.ldx = x.stride(0); a.rows = x.size(0); a.cols = (int)cols;
+  a.ldg = gr.stride(0); a.ldx = xr.stride(0); a.rows = xr.size(0); a.cols = (int)cols;
   a.st = at::cuda::getCurrentCUDAStream();
   a.blocks = dispatch(a, x.scalar_type(), wt, true);
   Tensor partial;
@@ -362,11 +454,15 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad, const Tens
   dispatch(a, x.scalar_type(), wt, false);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (want_params) {
-    const dim3 grid((unsigned)((2 * cols + 31) / 32)), block(32, 32);
     auto fold = [&](auto acc, auto wv) {
       using A = decltype(acc);
       using W = decltype(wv);
-      layer_norm_fold_kernel<A, W><<<grid, block, 0, a.st>>>((const A*)a.partial, a.blocks, (int)cols, (W*)dw.data_ptr(), (W*)db.data_ptr());
+      if (cols >= 1024)
+        layer_norm_fold_kernel<A, W, 32><<<(unsigned)((2 * cols + 31) / 32), 1024, 0, a.st>>>((const A*)a.partial, a.blocks, (int)cols,
+                                                                                             (W*)dw.data_ptr(), (W*)db.data_ptr());
+      else
+        layer_norm_fold_kernel<A, W, 8><<<(unsigned)((2 * cols + 7) / 8), 1024, 0, a.st>>>((const A*)a.partial, a.blocks, (int)cols,
+                                                                                          (W*)dw.data_ptr(), (W*)db.data_ptr());
     };
     if (st == at::kDouble) fold(double{}, double{});
     else if (wt == at::kFloat) fold(float{}, float{});
@@ -380,6 +476,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad, const Tens
 }  // namespace nva
 
 TORCH_LIBRARY_FRAGMENT(nvalchemi, m) {
-  m.def("layer_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, float eps, bool stats) -> (Tensor, Tensor, Tensor)", &nva::layer_norm_fwd);
+  m.def("layer_norm_apply(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", &nva::layer_norm_apply);
+  m.def("layer_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)", &nva::layer_norm_fwd);
   m.def("layer_norm_bwd(Tensor grad, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, bool want_params, ScalarType? param_type) -> (Tensor, Tensor, Tensor)", &nva::layer_norm_bwd);
 }

@@ -153,12 +153,13 @@ def check(op: str, schema: Any, args: tuple, kwargs: dict) -> None:
 
 def wrap(name: str, fn: Callable) -> Callable:
     """Operator callable that validates first while the mode is on (used by the operator proxy)."""
-    schema = fn.default._schema
+    call = fn.default  # the only overload; calling it directly spares the search for it on every call
+    schema = call._schema
 
     def checked(*a: Any, **k: Any) -> Any:
         if _enabled:
             check(name, schema, a, k)
-        return fn(*a, **k)
+        return call(*a, **k)
 
     checked.__name__ = name
     return checked

@@ -23,7 +23,7 @@ ACTIVATIONS = {"silu": 0, "gelu": 1}  # gelu: g * Phi(g), by the error function
 _CUDA_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str) -> int:
+def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str) -> None:
     if activation not in ACTIVATIONS:
         raise ValueError(f"gated_feed_forward: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
     if x.dim() < 1 or any(w.dim() != 2 for w in (w_gate, w_up, w_down)):
@@ -42,7 +42,6 @@ def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: to
     if not x.dtype.is_floating_point or (x.is_cuda and x.dtype not in _CUDA_TYPES):
         raise TypeError(f"gated_feed_forward: {x.dtype} is not supported on {x.device.type}"
                         + (" (float32, bfloat16, float16)" if x.is_cuda else ""))
-    return ACTIVATIONS[activation]
 
 
 def _wide(t: torch.Tensor) -> torch.Tensor:
@@ -79,17 +78,35 @@ def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch
                                 ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
     """``(dx, dw_gate, dw_up, dw_down)`` for the gradient ``dy`` of ``y``; nothing of the forward pass is needed.
     ``input_grad=False`` / ``weight_grads=False`` leave the first / the other three out (``None``)."""
-    act = _check(x, w_gate, w_up, w_down, activation)
+    with torch.no_grad():
+        if x.is_cuda:
+            try:
+                dx, *dw = _nops.gated_ff_bwd(dy, x, w_gate, w_up, w_down, ACTIVATIONS.get(activation, -1),
+                                             (1 if input_grad else 0) | (6 if weight_grads else 0))
+            except RuntimeError:  # the operator refuses what the checks refuse; they say it in Python's exceptions
+                _check_backward(dy, x, w_gate, w_up, w_down, activation)
+                raise
+        else:
+            _check_backward(dy, x, w_gate, w_up, w_down, activation)
+            dx, *dw = (t.to(x.dtype) for t in _backward_formula(dy.reshape(-1, w_down.shape[1]), x.reshape(-1, x.shape[-1]), w_gate, w_up,
+                                                                w_down, activation))
+            dx = dx.reshape(x.shape)
+        return (dx if input_grad else None, *(dw if weight_grads else (None,) * 3))
+
+
+def _check_backward(dy, x, w_gate, w_up, w_down, activation) -> None:
+    _check(x, w_gate, w_up, w_down, activation)
     if dy.shape != (*x.shape[:-1], w_down.shape[1]) or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError(f"gated_feed_forward_backward: dy ({tuple(dy.shape)}, {dy.dtype}, {dy.device}) does not match y "
                          f"({(*x.shape[:-1], w_down.shape[1])}, {x.dtype}, {x.device})")
-    with torch.no_grad():
-        x2, dy2 = x.reshape(-1, x.shape[-1]), dy.reshape(-1, w_down.shape[1])
-        if not x.is_cuda:
-            dx, *dw = (t.to(x.dtype) for t in _backward_formula(dy2, x2, w_gate, w_up, w_down, activation))
-        else:
-            dx, *dw = _nops.gated_ff_bwd(dy2, x2, w_gate, w_up, w_down, act, (1 if input_grad else 0) | (6 if weight_grads else 0))
-        return (dx.reshape(x.shape) if input_grad else None, *(dw if weight_grads else (None,) * 3))
+
+
+def _forward_kernel(x, w_gate, w_up, w_down, activation):
+    try:
+        return _nops.gated_ff_fwd(x, w_gate, w_up, w_down, ACTIVATIONS.get(activation, -1))
+    except RuntimeError:
+        _check(x, w_gate, w_up, w_down, activation)
+        raise
 
 
 class _GatedFeedForward(torch.autograd.Function):
@@ -97,7 +114,7 @@ class _GatedFeedForward(torch.autograd.Function):
     def forward(ctx, x, w_gate, w_up, w_down, activation):
         ctx.save_for_backward(x, w_gate, w_up, w_down)
         ctx.activation = activation
-        return _nops.gated_ff_fwd(x, w_gate, w_up, w_down, ACTIVATIONS[activation])
+        return _forward_kernel(x, w_gate, w_up, w_down, activation)
 
     @staticmethod
     def backward(ctx, dy):
@@ -121,7 +138,9 @@ class _GatedFeedForwardGrad(torch.autograd.Function):
         again = torch.is_grad_enabled()  # a third derivative is wanted: keep the graph of this one
         with torch.enable_grad():
             args = [t if again else t.detach().requires_grad_(n) for t, n in zip(saved, need)]
-            outs = _backward_formula(*args, ctx.activation)
+            dy, x = args[:2]
+            dx, *dw = _backward_formula(dy.reshape(-1, dy.shape[-1]), x.reshape(-1, x.shape[-1]), *args[2:], ctx.activation)
+            outs = (dx.reshape(x.shape), *dw)
             pairs = [(o, d) for o, d in zip(outs, dd) if d is not None and o.requires_grad]
             wanted = [t for t, n in zip(args, need) if n]
             got = torch.autograd.grad([o for o, _ in pairs], wanted, [d.to(o.dtype) for o, d in pairs], create_graph=again,
@@ -138,16 +157,12 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     if torch.is_autocast_enabled(x.device.type):
         dt = torch.get_autocast_dtype(x.device.type)
         x, w_gate, w_up, w_down = (t.to(dt) for t in (x, w_gate, w_up, w_down))
-    act = _check(x, w_gate, w_up, w_down, activation)
     if not x.is_cuda:
+        _check(x, w_gate, w_up, w_down, activation)
         return _forward_formula(x, w_gate, w_up, w_down, activation)
-    _native.require(x)
-    x2 = x.reshape(-1, x.shape[-1])
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
-        y = _GatedFeedForward.apply(x2, w_gate, w_up, w_down, activation)
-    else:
-        y = _nops.gated_ff_fwd(x2, w_gate, w_up, w_down, act)
-    return y.reshape(*x.shape[:-1], w_down.shape[1])
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+        return _GatedFeedForward.apply(x, w_gate, w_up, w_down, activation)
+    return _forward_kernel(x, w_gate, w_up, w_down, activation)
 
 
 def check_errors(like: torch.Tensor) -> int:

@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import torch
 
-from nvalchemi_toolkit_b200.ops import _native
 from nvalchemi_toolkit_b200.ops._native_counter import ops as _nops
 
 MAX_COLS = 8192
@@ -38,16 +37,6 @@ def _check(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | No
                             + ("" if x.dtype == torch.float64 else " or float32"))
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"layer_norm: weight ({weight.dtype}) and bias ({bias.dtype}) must have one type")
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as a matrix with contiguous rows; a view wherever the strides allow one."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
-
-
-def _vec(t: torch.Tensor | None) -> torch.Tensor | None:
-    return None if t is None else t.contiguous()
 
 
 def _wide(t: torch.Tensor) -> torch.Tensor:
@@ -83,12 +72,15 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias
                        eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(y, mean, rstd)``: the normalised rows and the statistics the backward pass takes, one value per row (float32;
     float64 rows: float64).  Not recorded by autograd."""
-    _check(x, weight, bias)
     with torch.no_grad():
-        if not x.is_cuda:
-            return _forward_formula(x, weight, bias, eps)
-        y, mean, rstd = _nops.layer_norm_fwd(_rows(x), _vec(weight), _vec(bias), float(eps), True)
-        return y.view(x.shape), mean, rstd
+        if x.is_cuda:
+            try:
+                return _nops.layer_norm_fwd(x, weight, bias, eps)
+            except RuntimeError:  # the operator refuses what _check refuses; _check says it in Python's exceptions
+                _check(x, weight, bias)
+                raise
+        _check(x, weight, bias)
+        return _forward_formula(x, weight, bias, eps)
 
 
 def layer_norm_backward(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -97,29 +89,36 @@ def layer_norm_backward(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor,
     """``(dx, dweight, dbias)`` for the gradient ``grad`` of ``y``.  The parameters' gradients have the type of ``weight``
     (without a weight: ``param_dtype``, by default that of ``x``); ``param_grads=False`` leaves them out (``None``).  Their
     sums over the rows are added in a fixed order: the same inputs give the same bits."""
+    ptype = weight.dtype if weight is not None else (param_dtype or x.dtype)
+    with torch.no_grad():
+        if x.is_cuda:
+            try:
+                dx, dw, db = _nops.layer_norm_bwd(grad, x, mean, rstd, weight, param_grads, ptype)
+            except RuntimeError:
+                _check_backward(grad, x, mean, rstd, weight, param_dtype)
+                raise
+            return (dx, dw, db) if param_grads else (dx, None, None)
+        _check_backward(grad, x, mean, rstd, weight, param_dtype)
+        n = x.shape[-1]
+        xf, g = _wide(x).reshape(-1, n), _wide(grad).reshape(-1, n)
+        xh = (xf - mean[:, None]) * rstd[:, None]
+        gw = g if weight is None else g * _wide(weight)
+        dx = rstd[:, None] * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
+        dx = dx.to(x.dtype).reshape(x.shape)
+        return (dx, (g * xh).sum(0).to(ptype), g.sum(0).to(ptype)) if param_grads else (dx, None, None)
+
+
+def _check_backward(grad, x, mean, rstd, weight, param_dtype) -> None:
     _check(x, weight, None)
     if grad.shape != x.shape or grad.dtype != x.dtype or grad.device != x.device:
         raise ValueError(f"layer_norm_backward: grad ({tuple(grad.shape)}, {grad.dtype}, {grad.device}) does not match x "
                          f"({tuple(x.shape)}, {x.dtype}, {x.device})")
     n_rows, stat_type = x.numel() // x.shape[-1], torch.float64 if x.dtype == torch.float64 else torch.float32
     for name, t in (("mean", mean), ("rstd", rstd)):
-        if t.shape != (n_rows,) or t.dtype != stat_type or t.device != x.device:
+        if t.shape != (n_rows,) or t.dtype != stat_type or t.device != x.device or not t.is_contiguous():
             raise ValueError(f"layer_norm_backward: {name} must be what layer_norm_forward returned for x")
     if param_dtype is not None and param_dtype not in (x.dtype, torch.float32):
         raise TypeError(f"layer_norm_backward: param_dtype {param_dtype} with x of type {x.dtype}")
-    ptype = weight.dtype if weight is not None else (param_dtype or x.dtype)
-    with torch.no_grad():
-        if not x.is_cuda:
-            n = x.shape[-1]
-            xf, g = _wide(x).reshape(-1, n), _wide(grad).reshape(-1, n)
-            xh = (xf - mean[:, None]) * rstd[:, None]
-            gw = g if weight is None else g * _wide(weight)
-            dx = rstd[:, None] * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
-            dx = dx.to(x.dtype).reshape(x.shape)
-            return (dx, (g * xh).sum(0).to(ptype), g.sum(0).to(ptype)) if param_grads else (dx, None, None)
-        dx, dw, db = _nops.layer_norm_bwd(_rows(grad), _rows(x), mean.contiguous(), rstd.contiguous(), _vec(weight),
-                                          bool(param_grads), ptype)
-        return dx.view(x.shape), dw if param_grads else None, db if param_grads else None
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -170,11 +169,14 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                ) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis, in the type of ``x``; differentiable (twice and
     more in ``x``, ``weight`` and ``grad``).  ``weight`` and ``bias`` may be absent and may be float32 beside 16-bit rows."""
-    _check(x, weight, bias)
-    wants = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
     if not x.is_cuda:
+        _check(x, weight, bias)
         return _forward_formula(x, weight, bias, eps)[0]
-    _native.require(x)
-    if wants:
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, float(eps))
-    return _nops.layer_norm_fwd(_rows(x), _vec(weight), _vec(bias), float(eps), False)[0].view(x.shape)
+    try:
+        return _nops.layer_norm_apply(x, weight, bias, eps)
+    except RuntimeError:
+        _check(x, weight, bias)
+        raise

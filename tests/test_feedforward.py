@@ -84,7 +84,8 @@ def _run(m, k, h, n, dtype, device, act="silu", layout=None):
 
 
 SHAPES = [(1, 1, 1, 1), (1, 64, 128, 64), (3, 5, 7, 2), (21, 64, 128, 64), (128, 64, 64, 64), (129, 72, 136, 40), (130, 65, 257, 129),
-          (300, 128, 512, 128), (1000, 200, 777, 200), (2, 1024, 512, 1024), (4097, 40, 24, 8), (17, 1000, 96, 33)]
+          (300, 128, 512, 128), (1000, 200, 777, 200), (2, 1024, 512, 1024), (4097, 40, 24, 8), (17, 1000, 96, 33),
+          (5, 120, 72, 56), (8, 513, 130, 96), (8, 2048, 512, 264), (1, 1024, 4096, 1024)]
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])

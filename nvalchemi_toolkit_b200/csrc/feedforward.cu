@@ -26,11 +26,25 @@ using namespace dense;
 
 enum Act : int { kSilu = 0, kGelu = 1 };
 
+// 2^x and 1 / x by the special function unit, one instruction each (subnormal results become 0; 2 and 1 ulp): the epilogues
+// below are bound by what they issue.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
 // act(g) and act'(g); EXACT: float32 results (library exponential and division), else the fast ones (1e-6 relative).
 template <bool EXACT, int ACT>
 __device__ __forceinline__ void activate(float g, float& a, float& da) {
   if constexpr (ACT == kSilu) {
-    const float s = EXACT ? 1.f / (1.f + expf(-g)) : __fdividef(1.f, 1.f + __expf(-g));
+    const float s = EXACT ? 1.f / (1.f + expf(-g)) : fast_rcp(1.f + fast_exp2(-kLog2e * g));
     a = g * s;
     da = s * (1.f + g * (1.f - s));
   } else if constexpr (EXACT) {  // g * Phi(g)
@@ -40,7 +54,7 @@ __device__ __forceinline__ void activate(float g, float& a, float& da) {
   } else {
     // erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), z >= 0: Hastings' approximation (Abramowitz and Stegun,
     // 7.1.26), off by at most 1.5e-7; its exponential is the derivative's as well
-    const float z = 0.70710678118654752f * fabsf(g), e = __expf(-0.5f * g * g), t = __fdividef(1.f, 1.f + 0.3275911f * z);
+    const float z = 0.70710678118654752f * fabsf(g), e = fast_exp2(-0.5f * kLog2e * g * g), t = fast_rcp(1.f + 0.3275911f * z);
     const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
     const float cdf = g < 0.f ? q : 1.f - q;
     a = g * cdf;

@@ -51,7 +51,6 @@ __global__ void __launch_bounds__(256) rows_by_k_kernel(const X* __restrict__ x,
   const int parts = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), c0 = (int)blockIdx.x / parts * COLS;
   const int k_lo = (int)((int64_t)k * rank / parts), k_hi = (int)((int64_t)k * (rank + 1) / parts);
   const int r0 = blockIdx.y * R, rows = min(R, total_rows - r0);
-  stage_rows<X, R>(xs, x + r0 * ldx, ldx, sx, rows, k_lo, k_hi);
   const int lc = threadIdx.x % kLanes, kr = threadIdx.x / kLanes, c = c0 + lc * VEC;
   constexpr int STEP = 256 / kLanes, U = 4;  // rows of the weights at a time, loads in flight per matrix
   float acc[MATS][R][VEC];
@@ -61,27 +60,35 @@ __global__ void __launch_bounds__(256) rows_by_k_kernel(const X* __restrict__ x,
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) acc[m][r][v] = 0.f;
-  if (c < n) {
-    for (int k0 = k_lo + kr; k0 < k_hi; k0 += U * STEP) {
-      Vec<T, VEC> a[U], b[U];
+  Vec<T, VEC> a[U], b[U];
+  auto load = [&](int k0) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kk = min(k0 + u * STEP, k_hi - 1);  // past the end: the last row again, times zero below
+    for (int u = 0; u < U; ++u) {
+      const int kk = min(k0 + u * STEP, k_hi - 1);  // past the end: the last row again, not used below
+      if (c < n) {
         a[u] = *reinterpret_cast<const Vec<T, VEC>*>(w0 + kk * ld0 + c);
         if constexpr (MATS == 2) b[u] = *reinterpret_cast<const Vec<T, VEC>*>(w1 + kk * ld1 + c);
       }
+    }
+  };
+  // The first weights are on their way before x is waited for: a second launch reads what the first one writes as x alone.
+  load(k_lo + kr);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  stage_rows<X, R>(xs, x + r0 * ldx, ldx, sx, rows, k_lo, k_hi);
+  for (int k0 = k_lo + kr; k0 < k_hi; k0 += U * STEP) {
+    if (k0 != k_lo + kr) load(k0);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kk = k0 + u * STEP;
-        if (kk < k_hi) {
+    for (int u = 0; u < U; ++u) {
+      const int kk = k0 + u * STEP;
+      if (kk < k_hi && c < n) {
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float xv = xs[(kk - k_lo) * R + r];
+        for (int r = 0; r < R; ++r) {
+          const float xv = xs[(kk - k_lo) * R + r];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-              acc[0][r][v] += xv * widen(a[u].v[v]);
-              if constexpr (MATS == 2) acc[1][r][v] += xv * widen(b[u].v[v]);
-            }
+          for (int v = 0; v < VEC; ++v) {
+            acc[0][r][v] += xv * widen(a[u].v[v]);
+            if constexpr (MATS == 2) acc[1][r][v] += xv * widen(b[u].v[v]);
           }
         }
       }
@@ -132,6 +139,8 @@ __global__ void __launch_bounds__(256) rows_by_n_kernel(const X* __restrict__ x,
                                                         int act, void* __restrict__ out, int64_t ldo, int out32) {
   extern __shared__ float xs[];
   const int r0 = blockIdx.y * R, rows = min(R, total_rows - r0);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   stage_rows<X, R>(xs, x + r0 * ldx, ldx, sx, rows, 0, k);
   const int col = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (col >= n) return;
@@ -193,11 +202,13 @@ void product(const X* x, int64_t ldx, int64_t sx, const Weight& a, const Weight&
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = (size_t)((k + parts - 1) / parts) * R * sizeof(float);
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)parts; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = MATS == 1 ? 2 : 1;  // the first launch reads weights before it waits: it must not start early itself
     C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, x, ldx, sx, (const T*)a.p, a.ld, (const T*)b.p, b.ld, rows, k, n, act, out, ldo, out32 ? 1 : 0));
   };
   if (!a.by_k) {

@@ -15,7 +15,8 @@
 // over several tiles.
 //
 // One persistent CTA per SM: warp 0 loads tiles by TMA into a ring of stages, one lane of warp 1 issues tcgen05.mma
-// (K = 16 per instruction), warps 2..9 are the epilogue.  The accumulator is double buffered (2 x 256 TMEM columns), so the
+// (K = 16 per instruction), warps 2..9 are the epilogue (16 warps
+// leave 96 registers a thread and were slower).  The accumulator is double buffered (2 x 256 TMEM columns), so the
 // epilogue of a tile runs beside the products of the next one; products with several accumulators use all of the TMEM for one
 // tile (their six passes hide the epilogue less, but it is a tenth of them).
 //
@@ -40,8 +41,8 @@ namespace nva {
 namespace dense {
 
 constexpr int BM = 128, BK = 64, kChunk = 64 * 64 * 2;  // a chunk: 64 x 64 16-bit values, one TMA box
-constexpr int kMaxSegs = 12, kMaxMaps = 6, kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kMaxSegs = 12, kMaxMaps = 6, kStaging = 32768;  // bytes of staging, shared by the epilogue's warps
+constexpr int kEpiWarps = 8, kThreads = 32 * (2 + kEpiWarps);
 
 static __device__ int error_word;
 
@@ -155,8 +156,12 @@ __device__ __forceinline__ void mma16(uint32_t d, uint64_t da, uint64_t db, uint
 // A stage of one CTA: 128 rows of A and the tile of B, or half of it in a pair.
 template <int BN, bool PAIR> constexpr int stage_bytes() { return (BM / 64 + BN / (PAIR ? 128 : 64)) * kChunk; }
 template <int BN, bool PAIR> constexpr int stage_count() { return 196608 / stage_bytes<BN, PAIR>(); }
-// ring + per-warp staging (32 rows of 128 bytes) + barriers, and slack for 1024-byte alignment
-template <int BN, bool PAIR> constexpr int smem_bytes() { return 1024 + stage_count<BN, PAIR>() * stage_bytes<BN, PAIR>() + kEpiWarps * 4096 + 512; }
+// ring + staging + barriers, and slack for 1024-byte alignment
+template <int BN, bool PAIR> constexpr int smem_bytes() { return 1024 + stage_count<BN, PAIR>() * stage_bytes<BN, PAIR>() + kStaging + 512; }
+
+// 16-byte slots of a staged row are turned by its number, so that eight consecutive rows' same slots lie in different banks.
+template <int SLOTS>
+__device__ __forceinline__ int turn_of(int row) { return (SLOTS == 8 ? row : SLOTS == 4 ? row >> 1 : row >> 2) & (SLOTS - 1); }
 
 // One warp's 32 rows x (SLOTS * 16) bytes from registers (lane = row) to global memory in whole row pieces: through shared
 // memory, 16-byte slots swizzled by row so that neither side has bank conflicts.  `cols_left`: elements of type T that exist
@@ -168,7 +173,7 @@ __device__ __forceinline__ void store_piece(uint4* stage, const uint4 (&v)[SLOTS
   constexpr int PER = 16 / (int)sizeof(T), RPI = 32 / SLOTS;
   if (cols_left <= 0) return;  // the same for the whole warp
 #pragma unroll
-  for (int j = 0; j < SLOTS; ++j) stage[lane * SLOTS + (j ^ (lane & (SLOTS - 1)))] = v[j];
+  for (int j = 0; j < SLOTS; ++j) stage[lane * SLOTS + (j ^ turn_of<SLOTS>(lane))] = v[j];
   __syncwarp();
   if (vec_ok && cols_left >= SLOTS * PER) {
     const int slot = lane % SLOTS, r0 = lane / SLOTS;
@@ -176,7 +181,7 @@ __device__ __forceinline__ void store_piece(uint4* stage, const uint4 (&v)[SLOTS
     for (int i = 0; i < SLOTS; ++i) {
       const int r = i * RPI + r0;
       if (r < rows_left)
-        *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + slot * PER) = stage[r * SLOTS + (slot ^ (r & (SLOTS - 1)))];
+        *reinterpret_cast<uint4*>(dst + (int64_t)r * ld + slot * PER) = stage[r * SLOTS + (slot ^ turn_of<SLOTS>(r))];
     }
   } else {  // rows off the 16-byte boundaries, or the last columns: a row at a time, an element a lane
     const T* const e = reinterpret_cast<const T*>(stage);
@@ -186,7 +191,7 @@ __device__ __forceinline__ void store_piece(uint4* stage, const uint4 (&v)[SLOTS
       const int j = c + lane, slot = j / PER, k = j % PER;
 #pragma unroll 8
       for (int r = 0; r < 32; ++r)
-        if (r < rows_left && j < cols_left) dst[(int64_t)r * ld + j] = e[(r * SLOTS + (slot ^ (r & (SLOTS - 1)))) * PER + k];
+        if (r < rows_left && j < cols_left) dst[(int64_t)r * ld + j] = e[(r * SLOTS + (slot ^ turn_of<SLOTS>(r))) * PER + k];
     }
   }
   __syncwarp();
@@ -212,11 +217,11 @@ __device__ __forceinline__ void turn_piece(uint4* stage, uint4 (&raw)[SLOTS]) {
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
     const int r = i * RPI + r0;
-    stage[r * SLOTS + (slot ^ (r & (SLOTS - 1)))] = raw[i];
+    stage[r * SLOTS + (slot ^ turn_of<SLOTS>(r))] = raw[i];
   }
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < SLOTS; ++j) raw[j] = stage[lane * SLOTS + (j ^ (lane & (SLOTS - 1)))];
+  for (int j = 0; j < SLOTS; ++j) raw[j] = stage[lane * SLOTS + (j ^ turn_of<SLOTS>(lane))];
   __syncwarp();
 }
 
@@ -275,8 +280,8 @@ __device__ __forceinline__ void acc_ld32(uint32_t tm, float (&v)[32], int used) 
 }
 
 // Epi::kAcc accumulators per column group, kStride columns apart; Epi::kLate: see below; Epi::Params; Epi::Pre: what
-// Epi::prefetch(params, tiles, tile, first row of the warp, half, pre) reads before the tile's products are done;
-// Epi::run(params, tiles, tile, tmem (lane quarter added), first row, half, stage, pre).
+// Epi::prefetch(params, tiles, tile, first row of the warp, share of the columns, pre) reads before the tile's products are done;
+// Epi::run(params, tiles, tile, tmem (lane quarter added), first row, share, stage, pre).
 //
 // kLate: a tile fills TMEM columns 0..383, group 0 in 0..255 and group 1 (whose segments come first) in the 128 columns after
 // those, in turns with the last 128, so that the next tile's group 1 is formed while the epilogue still reads this tile.
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int ACC = Epi::kAcc, BUFS = ACC == 1 && !Epi::kLate ? 2 : 1, CTAS = PAIR ? 2 : 1;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const generic = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t bar0 = base + STAGES * STAGE + kEpiWarps * 4096;
+  const uint32_t bar0 = base + STAGES * STAGE + kStaging;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
   auto acc_full = [&](int s) { return bar0 + 8u * (2 * STAGES + s); };
@@ -384,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int sg = 0; sg < t.n_seg && ok; ++sg) {
           const Seg s = t.seg[sg];
           if (!free && (!Epi::kLate || s.group == 0)) {
-            ok = mbar_wait_cluster(acc_empty(as), ((seq / BUFS) & 1) ^ 1, err, 12);
+            ok = mbar_wait(acc_empty(as), ((seq / BUFS) & 1) ^ 1, err, 12);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             free = true;
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t ka = (s.a_mn ? 2048 : 32) >> 4, kb_step = (s.b_mn ? 2048 : 32) >> 4;
           const uint32_t d0 = tmem + as * 256 + s.col + (Epi::kLate && s.group == 1 ? (seq & 1) * 128 : 0);
           for (int kb = lo; kb < hi; ++kb) {
-            if (!mbar_wait_cluster(full(st), phase, err, 13)) { ok = false; break; }
+            if (!mbar_wait(full(st), phase, err, 13)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint64_t da = da0 + (uint32_t)(st * (int)(STAGE >> 4)), db = db0 + (uint32_t)(st * (int)(STAGE >> 4));
             const int j = ACC > 1 && s.spread ? (kb - lo) % ACC : 0;
@@ -413,17 +418,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    const int w = warp - 2, q = warp & 3, half = w >> 2;  // q: the TMEM lanes this warp may read
-    uint4* const stage = reinterpret_cast<uint4*>(generic + STAGES * STAGE + w * 4096);
+    const int w = warp - 2, q = warp & 3;  // q: the TMEM lanes this warp may read
+    const int part = w >> 2;                        // its half of the columns
+    uint4* const stage = reinterpret_cast<uint4*>(generic + STAGES * STAGE + w * (kStaging / kEpiWarps));
     int seq = 0;
     for (int i = first_tile; i < t.total; i += tile_step, ++seq) {
       const TileAt at = tile_at(t, i, seq);
       const int as = BUFS == 2 ? seq & 1 : 0, row0 = at.m * (BM * CTAS) + (int)rank * BM + q * 32;
       typename Epi::Pre pre;
-      Epi::prefetch(ep, t, at, row0, half, pre);
-      if (!mbar_wait_cluster(acc_full(as), (seq / BUFS) & 1, err, 15)) break;
+      Epi::prefetch(ep, t, at, row0, part, pre);
+      if (!mbar_wait(acc_full(as), (seq / BUFS) & 1, err, 15)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      Epi::run(ep, t, at, tmem + as * 256 + ((uint32_t)(q * 32) << 16), row0, half, stage, pre);
+      Epi::run(ep, t, at, tmem + as * 256 + ((uint32_t)(q * 32) << 16), row0, part, stage, pre);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
@@ -455,14 +461,15 @@ struct EpiStore : NoPrefetch {
   static constexpr bool kLate = false;
   static_assert(ACC == 1 || ACC * BN <= 512, "dense: accumulators exceed the TMEM");
   struct Params { T* out; int64_t ld, batch_stride, split_stride; float alpha; };
-  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
+  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
+    constexpr int COLS = BN / 2;  // columns of a warp
     T* out = p.out + at.batch * p.batch_stride + at.split * p.split_stride;
     const bool vec_ok = p.ld % (16 / (int)sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     const int used = used_acc<ACC>(t, at, 0);
 #pragma unroll 1
-    for (int cb = 0; cb < BN / 64; ++cb) {
-      const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c;
+    for (int cb = 0; cb < COLS / 32; ++cb) {
+      const int c = part * COLS + cb * 32, n0 = at.n * BN + c;
       float v[32];
       acc_ld32<ACC, BN>(tm + c, v, used);
 #pragma unroll

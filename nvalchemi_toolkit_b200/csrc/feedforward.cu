@@ -62,22 +62,22 @@ __device__ __forceinline__ void activate(float g, float& a, float& da) {
   }
 }
 
-// The branch on the activation stays outside the loop over a thread's 32 values: inside it the values' chains of dependent
+// The branch on the activation stays outside the loop over a thread's values: inside it the values' chains of dependent
 // instructions would run one after the other (131,072 x 128 x 512: 222 us that way).
-template <bool EXACT, int ACT>
-__device__ __forceinline__ void gate32(float (&g)[32], const float (&u)[32]) {
+template <bool EXACT, int ACT, int C>
+__device__ __forceinline__ void gate(float (&g)[C], const float (&u)[C]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
+  for (int j = 0; j < C; ++j) {
     float a, da;
     activate<EXACT, ACT>(g[j], a, da);
     g[j] = a * u[j];
   }
 }
 // (g, u, dh) -> (dg, h, du)
-template <bool EXACT, int ACT>
-__device__ __forceinline__ void gate_grad32(float (&g)[32], float (&u)[32], float (&d)[32]) {
+template <bool EXACT, int ACT, int C>
+__device__ __forceinline__ void gate_grad(float (&g)[C], float (&u)[C], float (&d)[C]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
+  for (int j = 0; j < C; ++j) {
     float a, da;
     activate<EXACT, ACT>(g[j], a, da);
     g[j] = d[j] * u[j] * da;
@@ -86,30 +86,43 @@ __device__ __forceinline__ void gate_grad32(float (&g)[32], float (&u)[32], floa
   }
 }
 
-// Stores 32 columns of a warp's 32 rows as T, or as three bf16 planes of a float32 value.
-template <typename T>
-__device__ __forceinline__ void store32(uint4* stage, float (&v)[32], void* dst, int64_t off, int64_t ld, int64_t plane, int rows_left,
-                                        int cols_left, bool vec_ok) {
-  if constexpr (sizeof(T) == 2) {
-    uint4 o[4];
-    pack32<T>(v, o);
-    store_piece<T, 4>(stage, o, (T*)dst + off, ld, rows_left, cols_left, vec_ok);
-  } else {
-    float p1[32], p2[32];
+// C columns (16 or 32) of a warp's 32 rows as T, or as three bf16 planes of a float32 value.
+template <typename T, int C>
+__device__ __forceinline__ void store_cols(uint4* stage, float (&v)[C], void* dst, int64_t off, int64_t ld, int64_t plane, int rows_left,
+                                           int cols_left) {
+  auto put = [&](const float (&f)[C], auto tag, int64_t at) {
+    using S = decltype(tag);
+    uint4 o[C / 8];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
+    for (int j = 0; j < C / 8; ++j)
+      o[j] = make_uint4(pack2(f[8 * j], f[8 * j + 1], S{}), pack2(f[8 * j + 2], f[8 * j + 3], S{}), pack2(f[8 * j + 4], f[8 * j + 5], S{}),
+                        pack2(f[8 * j + 6], f[8 * j + 7], S{}));
+    store_piece<S, C / 8>(stage, o, (S*)dst + at, ld, rows_left, cols_left, true);  // rows are padded to 8
+  };
+  if constexpr (sizeof(T) == 2) {
+    put(v, T{}, off);
+  } else {
+    float p1[C], p2[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
       float a, b, c;
       split3(v[j], a, b, c);
       v[j] = a; p1[j] = b; p2[j] = c;
     }
-    uint4 o[4];
-    __nv_bfloat16* d = (__nv_bfloat16*)dst + off;
-    pack32<__nv_bfloat16>(v, o);
-    store_piece<__nv_bfloat16, 4>(stage, o, d, ld, rows_left, cols_left, vec_ok);
-    pack32<__nv_bfloat16>(p1, o);
-    store_piece<__nv_bfloat16, 4>(stage, o, d + plane, ld, rows_left, cols_left, vec_ok);
-    pack32<__nv_bfloat16>(p2, o);
-    store_piece<__nv_bfloat16, 4>(stage, o, d + 2 * plane, ld, rows_left, cols_left, vec_ok);
+    put(v, __nv_bfloat16{}, off);
+    put(p1, __nv_bfloat16{}, off + plane);
+    put(p2, __nv_bfloat16{}, off + 2 * plane);
+  }
+}
+
+// C columns of the accumulator (of several, see acc_ld32).
+template <int C, int ACC, int STRIDE>
+__device__ __forceinline__ void acc_ld(uint32_t tm, float (&v)[C], int used) {
+  if constexpr (C == 32) {
+    acc_ld32<ACC, STRIDE>(tm, v, used);
+  } else {
+    static_assert(C == 16 && ACC == 1, "dense: 16 columns of one accumulator");
+    tmem_ld16(tm, v);
   }
 }
 
@@ -119,18 +132,19 @@ struct EpiGated : NoPrefetch {
   static constexpr int kAcc = sizeof(T) == 4 ? 512 / BN : 1, kStride = BN;
   static constexpr bool kLate = false;
   struct Params { void* h; int64_t ld, plane; int act; };
-  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
+  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
+    constexpr int COLS = BN / 4, C = 32;
     const int used = used_acc<kAcc>(t, at, 0);
 #pragma unroll 1
-    for (int cb = 0; cb < BN / 128; ++cb) {
-      const int c = half * (BN / 4) + cb * 32, n0 = at.n * (BN / 2) + c;
-      float g[32], u[32];
-      acc_ld32<kAcc, kStride>(tm + c, g, used);
-      acc_ld32<kAcc, kStride>(tm + BN / 2 + c, u, used);
-      if (p.act == kSilu) gate32<sizeof(T) == 4, kSilu>(g, u);
-      else gate32<sizeof(T) == 4, kGelu>(g, u);
-      store32<T>(stage, g, p.h, (int64_t)row0 * p.ld + n0, p.ld, p.plane, t.M - row0, t.N - n0, true);
+    for (int cb = 0; cb < COLS / C; ++cb) {
+      const int c = part * COLS + cb * C, n0 = at.n * (BN / 2) + c;
+      float g[C], u[C];
+      acc_ld<C, kAcc, kStride>(tm + c, g, used);
+      acc_ld<C, kAcc, kStride>(tm + BN / 2 + c, u, used);
+      if (p.act == kSilu) gate<sizeof(T) == 4, kSilu>(g, u);
+      else gate<sizeof(T) == 4, kGelu>(g, u);
+      store_cols<T>(stage, g, p.h, (int64_t)row0 * p.ld + n0, p.ld, p.plane, t.M - row0, t.N - n0);
     }
   }
 };
@@ -143,23 +157,24 @@ struct EpiGatedGrad : NoPrefetch {
   static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1, kStride = 192;
   static constexpr bool kLate = sizeof(T) == 2;
   struct Params { void *dg, *du, *h; int64_t ld, plane; int act; };
-  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
+  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
+    constexpr int COLS = kHc / 2, C = 32;
     const int used = used_acc<kAcc>(t, at, 0), used1 = used_acc<kAcc>(t, at, 1);
     const uint32_t td = tm + 2 * kHc + (kLate ? (at.seq & 1) * 128 : 0);
 #pragma unroll 1
-    for (int cb = 0; cb < kHc / 64; ++cb) {
-      const int c = half * (kHc / 2) + cb * 32, n0 = at.n * kHc + c;
-      float g[32], u[32], d[32];
-      acc_ld32<kAcc, kStride>(tm + c, g, used);
-      acc_ld32<kAcc, kStride>(tm + kHc + c, u, used);
-      acc_ld32<kAcc, kStride>(td + c, d, used1);
-      if (p.act == kSilu) gate_grad32<sizeof(T) == 4, kSilu>(g, u, d);
-      else gate_grad32<sizeof(T) == 4, kGelu>(g, u, d);
+    for (int cb = 0; cb < COLS / C; ++cb) {
+      const int c = part * COLS + cb * C, n0 = at.n * kHc + c;
+      float g[C], u[C], d[C];
+      acc_ld<C, kAcc, kStride>(tm + c, g, used);
+      acc_ld<C, kAcc, kStride>(tm + kHc + c, u, used);
+      acc_ld<C, kAcc, kStride>(td + c, d, used1);
+      if (p.act == kSilu) gate_grad<sizeof(T) == 4, kSilu>(g, u, d);
+      else gate_grad<sizeof(T) == 4, kGelu>(g, u, d);
       const int64_t off = (int64_t)row0 * p.ld + n0;
-      store32<T>(stage, g, p.dg, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
-      store32<T>(stage, d, p.du, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
-      store32<T>(stage, u, p.h, off, p.ld, p.plane, t.M - row0, t.N - n0, true);
+      store_cols<T>(stage, g, p.dg, off, p.ld, p.plane, t.M - row0, t.N - n0);
+      store_cols<T>(stage, d, p.du, off, p.ld, p.plane, t.M - row0, t.N - n0);
+      store_cols<T>(stage, u, p.h, off, p.ld, p.plane, t.M - row0, t.N - n0);
     }
   }
 };

@@ -149,13 +149,13 @@ struct EpiGated : NoPrefetch {
   }
 };
 
-// Of HC columns of h: g in accumulator columns [0, HC), u in [HC, 2 HC), dh after those.  16 bits: 128 columns, dh in turns in
-// two places (see dense_kernel); float32: 64 columns, two accumulators each.
-template <typename T>
+// Of HC columns of h: g in accumulator columns [0, HC), u in [HC, 2 HC), dh after those.  One accumulator each: 128 columns, dh in
+// turns in two places (see dense_kernel).  Two accumulators, for float32 sums of more than 512 terms: 64 columns.
+template <typename T, int ACC>
 struct EpiGatedGrad : NoPrefetch {
-  static constexpr int kHc = sizeof(T) == 4 ? 64 : 128;
-  static constexpr int kAcc = sizeof(T) == 4 ? 2 : 1, kStride = 192;
-  static constexpr bool kLate = sizeof(T) == 2;
+  static constexpr int kHc = ACC == 2 ? 64 : 128;
+  static constexpr int kAcc = ACC, kStride = 192;
+  static constexpr bool kLate = ACC == 1;
   struct Params { void *dg, *du, *h; int64_t ld, plane; int act; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
@@ -179,16 +179,21 @@ struct EpiGatedGrad : NoPrefetch {
   }
 };
 
-// Copies a matrix into rows on 16-byte boundaries (T 16-bit), or splits float32 into three bf16 planes.  Two elements a thread.
+// Copies matrices into rows on 16-byte boundaries (T 16-bit), or splits float32 into three bf16 planes: one launch for all of a
+// call's operands (grid.y), two elements a thread.
+constexpr int kMaxPacks = 5;
+struct PackJob { const void* src; uint16_t* dst; int64_t ld, rows, cols, ldp, plane; };
+struct PackJobs { PackJob j[kMaxPacks]; int n = 0; };
+
 template <typename T, int P>
-__global__ void pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ dst,
-                            int64_t ldp, int64_t plane) {
-  const int64_t half = (cols + 1) / 2;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < rows * half; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / half, c = (i - r * half) * 2;
-    const bool two = c + 1 < cols;
-    const T* s = src + r * ld + c;
-    uint16_t* d = dst + r * ldp + c;
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
+  const PackJob job = jobs.j[blockIdx.y];
+  const int64_t half = (job.cols + 1) / 2, total = job.rows * half;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = total <= 0x7fffffff ? (int64_t)((uint32_t)i / (uint32_t)half) : i / half, c = (i - r * half) * 2;
+    const bool two = c + 1 < job.cols;
+    const T* s = (const T*)job.src + r * job.ld + c;
+    uint16_t* d = job.dst + r * job.ldp + c;
     if constexpr (P == 1) {
       const uint16_t* s16 = reinterpret_cast<const uint16_t*>(s);
       *reinterpret_cast<uint32_t*>(d) = (uint32_t)s16[0] | (two ? (uint32_t)s16[1] << 16 : 0u);
@@ -197,9 +202,19 @@ __global__ void pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows,
       split3((float)s[0], a[0], a[1], a[2]);
       if (two) split3((float)s[1], b[0], b[1], b[2]);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(d + k * plane) = pack2(a[k], b[k], __nv_bfloat16{});
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(d + k * job.plane) = pack2(a[k], b[k], __nv_bfloat16{});
     }
   }
+}
+
+void run_packs(const PackJobs& jobs, int planes, cudaStream_t st) {
+  if (jobs.n == 0) return;
+  int64_t most = 0;
+  for (int i = 0; i < jobs.n; ++i) most = std::max(most, jobs.j[i].rows * ((jobs.j[i].cols + 1) / 2));
+  const dim3 grid((unsigned)std::min<int64_t>((most + 255) / 256, 148 * 8), (unsigned)jobs.n);
+  if (planes == 3) pack_kernel<float, 3><<<grid, 256, 0, st>>>(jobs);
+  else pack_kernel<__half, 1><<<grid, 256, 0, st>>>(jobs);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 // out = sum over splits of partial [splits][n], in order.
@@ -216,7 +231,7 @@ __global__ void split_sum_kernel(const float* __restrict__ partial, int splits, 
 // runs over axis `k_axis` of the logical matrix.
 struct Operand {
   Stored s;
-  Tensor keep;
+  Tensor keep, source;
   bool rowmajor = true;
   bool mn(int k_axis) const { return rowmajor != (k_axis == 1); }
   int64_t extent(int axis) const { return (axis == 1) == rowmajor ? s.inner : s.outer; }
@@ -224,12 +239,15 @@ struct Operand {
 
 int planes_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? 3 : 1; }
 
-Operand operand(Tensor t, cudaStream_t st) {
+// Whether a matrix is read by rows (its columns contiguous otherwise); one with neither axis contiguous is copied by rows.
+bool by_rows(const Tensor& t) { return t.stride(1) == 1 || t.size(1) == 1 || !(t.stride(0) == 1 || t.size(0) == 1); }
+
+// The operand of a tensor, read by rows or by columns; what has to be packed for it is added to `jobs` and there after run_packs.
+Operand operand(Tensor t, PackJobs& jobs, bool rowmajor) {
   Operand o;
-  if (t.stride(1) != 1 && t.size(1) != 1) {
-    if (t.stride(0) == 1 || t.size(0) == 1) { t = t.t(); o.rowmajor = false; }
-    else t = t.contiguous();
-  }
+  o.rowmajor = rowmajor;
+  if (!rowmajor) t = t.t();
+  if (t.stride(1) != 1 && t.size(1) != 1) t = t.contiguous();
   const int64_t rows = t.size(0), cols = t.size(1), ld = rows > 1 ? t.stride(0) : cols;
   if (planes_of(t) == 1 && (rows == 1 || (ld % 8 == 0 && ld >= cols)) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) {
     o.keep = t;
@@ -238,16 +256,14 @@ Operand operand(Tensor t, cudaStream_t st) {
   }
   const int P = planes_of(t);
   const int64_t ldp = (cols + 7) / 8 * 8;
+  o.source = t;
   o.keep = at::empty({P, rows, ldp}, t.options().dtype(P == 3 ? at::kBFloat16 : t.scalar_type()));
-  const int64_t work = rows * ((cols + 1) / 2);
-  const unsigned grid = (unsigned)std::min<int64_t>((work + 255) / 256, 148 * 16);
-  uint16_t* d = (uint16_t*)o.keep.data_ptr();
-  if (P == 3) pack_kernel<float, 3><<<grid, 256, 0, st>>>(t.data_ptr<float>(), ld, rows, cols, d, ldp, rows * ldp);
-  else pack_kernel<__half, 1><<<grid, 256, 0, st>>>((const __half*)t.data_ptr(), ld, rows, cols, d, ldp, 0);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  TORCH_CHECK(jobs.n < kMaxPacks, "gated_ff: too many operands to pack");
+  jobs.j[jobs.n++] = {t.data_ptr(), (uint16_t*)o.keep.data_ptr(), ld, rows, cols, ldp, rows * ldp};
   o.s = {o.keep.data_ptr(), cols, rows, ldp, P, rows * ldp};
   return o;
 }
+Operand operand(const Tensor& t, PackJobs& jobs) { return operand(t, jobs, by_rows(t)); }
 
 // Intermediate [P][rows][ld] (16-bit) that epilogues write and later products read.
 Operand intermediate(int64_t rows, int64_t cols, int P, const Tensor& like, int copies = 1) {
@@ -290,14 +306,14 @@ struct Plan {
 };
 
 // Plain product into `out` [batches][M][N].  The contraction axis is split over several tiles (partials added in order by a
-// second kernel) when there are fewer tiles than the GPU runs at a time and the axis is long, and for float32 so that no
-// accumulator takes more than 32 instructions of the large partial product.
+// second kernel) when half of the GPU or more would have no tile and the axis is long, and for float32 so that no accumulator
+// takes more than 32 instructions of the large partial product.
 template <typename T, int BN, int ACC>
 void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   set_tiles(pl.t, M, N, BN, batches, 1);
   const int tiles = pl.t.total, nk = pl.t.main_nk[0], kb = nk * pl.t.n_seg, at_once = slots(pl.t);
   int splits = 1;
-  if (tiles < at_once) splits = std::max(1, std::min({2 * at_once / tiles, kb / 8, nk, 64}));
+  if (2 * tiles <= at_once) splits = std::max(1, std::min({at_once / tiles, kb / 8, nk, 64}));
   if (ACC > 1) splits = std::max(splits, (nk + 8 * ACC - 1) / (8 * ACC));
   if (splits == 1) {
     typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
@@ -314,17 +330,17 @@ void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N,
 }
 
 // Columns of a tile of an M x N product.
-int store_bn(int P, int64_t batches, int64_t M, int64_t N) {
-  if (P != 1 || !use_pair(M)) return 128;
+int store_bn(int64_t batches, int64_t M, int64_t N) {
+  if (!use_pair(M)) return 128;
   const int64_t rows = batches * ((M + 2 * BM - 1) / (2 * BM));
   return pick_bn(rows * ((N + 255) / 256), rows * ((N + 127) / 128));
 }
 void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   auto go = [&](auto v) {
     using T = decltype(v);
-    if constexpr (sizeof(T) == 4) store_product<T, 128, 4>(pl, out, batches, M, N, st);
-    else if (bn == 256) store_product<T, 256, 1>(pl, out, batches, M, N, st);
-    else store_product<T, 128, 1>(pl, out, batches, M, N, st);
+    constexpr int ACC = sizeof(T) == 4 ? 2 : 1;  // float32: all of the TMEM
+    if (bn == 256) store_product<T, 256, ACC>(pl, out, batches, M, N, st);
+    else store_product<T, 128, 2 * ACC - (ACC == 1)>(pl, out, batches, M, N, st);
   };
   if (out.scalar_type() == at::kFloat) go(float{});
   else if (out.scalar_type() == at::kHalf) go(__half{});
@@ -363,8 +379,9 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
   if (gated_ff_rows(x, wg, wu, wd, act, y, st)) return y;
   const int P = planes_of(x);
   const bool bf16 = x.scalar_type() != at::kHalf;
-  Operand ox = operand(x, st), og = operand(wg, st), ou = operand(wu, st), od = operand(wd, st);
-  if (og.rowmajor != ou.rowmajor) ou = operand(og.rowmajor ? wu.contiguous() : wu.t().contiguous().t(), st);
+  PackJobs jobs;
+  Operand ox = operand(x, jobs), og = operand(wg, jobs), ou = operand(wu, jobs, og.rowmajor), od = operand(wd, jobs);
+  run_packs(jobs, P, st);
   Operand oh = intermediate(M, H, P, x);
   {
     Plan pl(P, bf16);
@@ -378,16 +395,15 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
       run_dense<BN, EpiGated<T, BN>>(pl.maps, pl.t, ep, st);
     };
     auto wide = [&](auto v) {
-      if constexpr (sizeof(v) == 2)
-        if (store_bn(P, 1, M, 2 * H) == 256) return go(v, std::integral_constant<int, 256>{});
-      go(v, std::integral_constant<int, 128>{});
+      if (store_bn(1, M, 2 * H) == 256) go(v, std::integral_constant<int, 256>{});
+      else go(v, std::integral_constant<int, 128>{});
     };
     if (P == 3) wide(float{});
     else if (bf16) wide(__nv_bfloat16{});
     else wide(__half{});
   }
   Plan pl(P, bf16);
-  const int bn = store_bn(P, 1, M, N);
+  const int bn = store_bn(1, M, N);
   const int a = pl.map(oh), b = pl.map(od);
   pl.product(a, oh, 1, b, -1, od, 0, 0, bn);
   store_any(pl, bn, y, 1, M, N, st);
@@ -413,29 +429,35 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
   }
   const int P = planes_of(x);
   const bool bf16 = x.scalar_type() != at::kHalf;
-  Operand ox = operand(x, st), og = operand(wg, st), ou = operand(wu, st), od = operand(wd, st), oy = operand(dy, st);
-  if (og.rowmajor != ou.rowmajor) ou = operand(og.rowmajor ? wu.contiguous() : wu.t().contiguous().t(), st);
+  PackJobs jobs;
+  Operand ox = operand(x, jobs), og = operand(wg, jobs), ou = operand(wu, jobs, og.rowmajor), od = operand(wd, jobs), oy = operand(dy, jobs);
+  run_packs(jobs, P, st);
   Operand oe = intermediate(M, H, P, x, 2), oh = intermediate(M, H, P, x);  // dg then du; h
   {
     Plan pl(P, bf16);
     const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou), a3 = pl.map(oy), b3 = pl.map(od);
-    const int hc = P == 3 ? 64 : 128;
-    pl.product(a3, oy, 1, b3, -1, od, 1, 2 * hc, hc, 0, 0, 0, 0, 2, 1);
-    pl.product(a, ox, 1, b, b2, og, 0, 0, 2 * hc);
-    set_tiles(pl.t, M, H, hc, 1, 1, false, P == 1);  // 64 columns of dh are too few for a pair
-    auto go = [&](auto v) {
+    const bool deep = P == 3 && std::max(K, N) > 512;
+    const int hc = deep ? 64 : 128;
+    for (int part = 0; part < 2; ++part) pl.product(a3, oy, 1, b3, -1, od, 1, 2 * hc, hc, 0, 0, 0, 0, part, 1);
+    for (int part = 0; part < 2; ++part) pl.product(a, ox, 1, b, b2, og, 0, 0, 2 * hc, 0, 0, 0, 0, part);
+    set_tiles(pl.t, M, H, hc, 1, 1, false, !deep);  // 64 columns of dh are too few for a pair
+    auto go = [&](auto v, auto acc) {
       using T = decltype(v);
+      constexpr int ACC = decltype(acc)::value;
+      using Epi = EpiGatedGrad<T, ACC>;
       uint16_t* e = (uint16_t*)oe.keep.data_ptr();
-      typename EpiGatedGrad<T>::Params ep{e, e + P * oe.s.plane, oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act};
-      run_dense<2 * EpiGatedGrad<T>::kHc, EpiGatedGrad<T>, sizeof(T) == 2>(pl.maps, pl.t, ep, st);
+      typename Epi::Params ep{e, e + P * oe.s.plane, oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act};
+      run_dense<2 * Epi::kHc, Epi, ACC == 1>(pl.maps, pl.t, ep, st);
     };
-    if (P == 3) go(float{});
-    else if (bf16) go(__nv_bfloat16{});
-    else go(__half{});
+    using One = std::integral_constant<int, 1>;
+    if (deep) go(float{}, std::integral_constant<int, 2>{});
+    else if (P == 3) go(float{}, One{});
+    else if (bf16) go(__nv_bfloat16{}, One{});
+    else go(__half{}, One{});
   }
   if (which & 1) {
     Plan pl(P, bf16);
-    const int bn = store_bn(P, 1, M, K);
+    const int bn = store_bn(1, M, K);
     const int a = pl.map(oe), b = pl.map(og), c = pl.map(ou);
     for (int part = 0; part < 2; ++part) {
       pl.product(a, oe, 1, b, -1, og, 1, 0, bn, 0, 0, 0, 0, part);
@@ -445,14 +467,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
   }
   if (which & 2) {
     Plan pl(P, bf16);
-    const int bn = store_bn(P, 2, K, H);
+    const int bn = store_bn(2, K, H);
     const int a = pl.map(ox), b = pl.map(oe);
     pl.product(a, ox, 0, b, -1, oe, 0, 0, bn, 0, 0, 0, P);
     store_any(pl, bn, dgu, 2, K, H, st);
   }
   if (which & 4) {
     Plan pl(P, bf16);
-    const int bn = store_bn(P, 1, H, N);
+    const int bn = store_bn(1, H, N);
     const int a = pl.map(oh), b = pl.map(oy);
     pl.product(a, oh, 0, b, -1, oy, 0, 0, bn);
     store_any(pl, bn, dwd, 1, H, N, st);

@@ -112,7 +112,7 @@ def test_large_products(m, k, h, n, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("layout", ["linear", "mixed", "sliced"])
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("m,k,h,n", [(200, 96, 160, 96), (3, 96, 160, 96), (77, 50, 90, 34)])
+@pytest.mark.parametrize("m,k,h,n", [(200, 96, 160, 96), (3, 96, 160, 96), (77, 50, 90, 34), (20, 1, 33, 1), (200, 1, 40, 7), (30, 16, 1, 16)])
 def test_layouts(m, k, h, n, dtype, layout):
     _run(m, k, h, n, dtype, "cuda", layout=layout)
 

@@ -329,12 +329,16 @@ void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N,
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// Columns of a tile of an M x N product.
-int store_bn(int64_t batches, int64_t M, int64_t N) {
+// Columns of a tile of an M x N product over `kb` blocks of the contraction axis (all segments): by the number of tiles, and 256
+// where splitting that axis fills at least three quarters of the GPU with wide tiles.
+int store_bn(int64_t batches, int64_t M, int64_t N, int64_t kb) {
   if (!use_pair(M)) return 128;
-  const int64_t rows = batches * ((M + 2 * BM - 1) / (2 * BM));
-  return pick_bn(rows * ((N + 255) / 256), rows * ((N + 127) / 128));
+  const int64_t rows = batches * ((M + 2 * BM - 1) / (2 * BM)), wide = rows * ((N + 255) / 256), pairs = sm_count() / 2;
+  if (wide < pairs && 4 * wide * std::min(pairs / wide, kb / 8) >= 3 * pairs) return 256;
+  return pick_bn(wide, rows * ((N + 127) / 128));
 }
+// Blocks of the contraction axis of a product with an axis of K.
+int64_t blocks_of(int P, int64_t K) { return (K + BK - 1) / BK * (P == 3 ? 6 : 1); }
 void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   auto go = [&](auto v) {
     using T = decltype(v);
@@ -395,7 +399,7 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
       run_dense<BN, EpiGated<T, BN>>(pl.maps, pl.t, ep, st);
     };
     auto wide = [&](auto v) {
-      if (store_bn(1, M, 2 * H) == 256) go(v, std::integral_constant<int, 256>{});
+      if (store_bn(1, M, 2 * H, 0) == 256) go(v, std::integral_constant<int, 256>{});
       else go(v, std::integral_constant<int, 128>{});
     };
     if (P == 3) wide(float{});
@@ -403,7 +407,7 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
     else wide(__half{});
   }
   Plan pl(P, bf16);
-  const int bn = store_bn(1, M, N);
+  const int bn = store_bn(1, M, N, blocks_of(P, H));
   const int a = pl.map(oh), b = pl.map(od);
   pl.product(a, oh, 1, b, -1, od, 0, 0, bn);
   store_any(pl, bn, y, 1, M, N, st);
@@ -457,7 +461,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
   }
   if (which & 1) {
     Plan pl(P, bf16);
-    const int bn = store_bn(1, M, K);
+    const int bn = store_bn(1, M, K, 2 * blocks_of(P, H));
     const int a = pl.map(oe), b = pl.map(og), c = pl.map(ou);
     for (int part = 0; part < 2; ++part) {
       pl.product(a, oe, 1, b, -1, og, 1, 0, bn, 0, 0, 0, 0, part);
@@ -467,14 +471,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
   }
   if (which & 2) {
     Plan pl(P, bf16);
-    const int bn = store_bn(2, K, H);
+    const int bn = store_bn(2, K, H, blocks_of(P, M));
     const int a = pl.map(ox), b = pl.map(oe);
     pl.product(a, ox, 0, b, -1, oe, 0, 0, bn, 0, 0, 0, P);
     store_any(pl, bn, dgu, 2, K, H, st);
   }
   if (which & 4) {
     Plan pl(P, bf16);
-    const int bn = store_bn(1, H, N);
+    const int bn = store_bn(1, H, N, blocks_of(P, M));
     const int a = pl.map(oh), b = pl.map(oy);
     pl.product(a, oh, 0, b, -1, oy, 0, 0, bn);
     store_any(pl, bn, dwd, 1, H, N, st);

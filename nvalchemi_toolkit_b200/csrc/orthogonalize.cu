@@ -266,7 +266,8 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const T* __restrict__ g, i
 // same bytes serve both; A and B share one 128 x 128 buffer.  A thread holds one row and half of the columns of every
 // accumulator; A stays in its registers in fp32 until B is formed.  X is kept as high + low part (22 bits), which for a
 // bfloat16 result is as good as fp32.  What bounds it is the chain of 15 products with an epilogue and two block barriers
-// between each: 24 matrices of 128 x 128 took 183 us as 17 launches.
+// between each; nothing of an epilogue may wait for its neighbour (conditions around shared-memory loads made B's 9400 clocks of
+// 19,000 a step).  24 matrices of 128 x 128 took 183 us as 17 launches.
 constexpr int kSmallThreads = 256, kSmallChunk = 128 * 128;  // bytes of 128 rows x 64 columns
 
 __device__ __forceinline__ uint32_t small_at(int row, int col) {  // byte offset of an element in a chunked, swizzled plane
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__(kSmallThreads)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   double s = 0.0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < count; i += kSmallThreads) {
     const double v = (double)widen(src[i]);
     s += v * v;
@@ -312,11 +314,19 @@ __global__ void __launch_bounds__(kSmallThreads)
   __syncthreads();
   s = 0.0;
   for (int i = 0; i < 8; ++i) s += part[i];
-  const double scale = 1.0 / (sqrt(s) + eps);
+  // 2^12 / (|G| + eps) as a mantissa and two powers of two, so that no factor leaves the fp32 range
+  int e;
+  const float mant = (float)frexp((double)kXScale / (sqrt(s) + eps), &e);
+  const float p1 = scalbnf(1.f, max(-126, min(127, e / 2))), p2 = scalbnf(1.f, max(-126, min(127, e - e / 2)));
+  const uint32_t magic = n > 1 ? (uint32_t)((0x100000000ull + n - 1) / n) : 0;  // i / n = umulhi(i, magic) for i < 2^16, n <= 256
+  auto place = [&](uint32_t i) {
+    const int gr = n > 1 ? (int)__umulhi(i, magic) : (int)i, gc = (int)i - gr * n;
+    return tall ? small_at(gc, gr) : small_at(gr, gc);
+  };
+#pragma unroll 4
   for (int i = threadIdx.x; i < count; i += kSmallThreads) {
-    const int gr = i / n, gc = i - gr * n;
-    const uint32_t at = tall ? small_at(gc, gr) : small_at(gr, gc);
-    const float v = (float)((double)widen(src[i]) * scale) * kXScale;
+    const uint32_t at = place(i);
+    const float v = widen(src[i]) * p1 * mant * p2;
     const __half h = __float2half_rn(v);
     *reinterpret_cast<__half*>(xh + at) = h;
     *reinterpret_cast<__half*>(xl + at) = __float2half_rn(v - __half2float(h));
@@ -392,17 +402,18 @@ __global__ void __launch_bounds__(kSmallThreads)
     }
     if (!done()) break;
     const float di = diag[row];
-    float bd = 0.f;
+    float aad = 0.f;  // the diagonal of R R
     auto poly = [&](float (&rv)[32], int base_col) {
       float v[32];
+      const float dl = diag[base_col + lane];
       tmem_ld32(t_gram + lanes + base_col, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        const int col = base_col + j;
-        const float aa = v[j] * (1.f / (kXScale * kXScale)), rij = rv[j] * (1.f / kXScale), dj = diag[col];
-        const bool on = row == col, in = col < r && row < r;
-        bd = on ? cb * di + cc * (di * di + aa) : bd;
-        rv[j] = on || !in ? 0.f : (cb * rij + cc * ((di + dj) * rij + aa)) * kBScale;
+        const float aa = v[j] * (1.f / (kXScale * kXScale)), rij = rv[j] * (1.f / kXScale);
+        const float b = cb * rij + cc * ((di + __shfl_sync(0xffffffffu, dl, j)) * rij + aa);
+        const bool on = row == base_col + j;
+        aad = on ? aa : aad;
+        rv[j] = on || base_col + j >= r ? 0.f : b * kBScale;  // columns past r hold nothing; rows past r are zero by themselves
       }
     };
     poly(a0, c0);
@@ -410,7 +421,7 @@ __global__ void __launch_bounds__(kSmallThreads)
     __syncthreads();  // R and the diagonal of A have been read
     put32(rb, c0, a0);
     put32(rb, c0 + 32, a1);
-    if (mine) diag[row] = bd;
+    if (mine) diag[row] = cb * di + cc * (di * di + aad);
     publish();
     if (threadIdx.x == 0) {  // B X: low part, high part
       for (int p = 0; p < 2; ++p)
@@ -455,10 +466,8 @@ __global__ void __launch_bounds__(kSmallThreads)
   }
   if (__syncthreads_and(ok)) {
     __nv_bfloat16* dst = out + blockIdx.x * (int64_t)count;
-    for (int i = threadIdx.x; i < count; i += kSmallThreads) {
-      const int gr = i / n, gc = i - gr * n;
-      dst[i] = *reinterpret_cast<const __nv_bfloat16*>(xh + (tall ? small_at(gc, gr) : small_at(gr, gc)));
-    }
+#pragma unroll 4
+    for (int i = threadIdx.x; i < count; i += kSmallThreads) dst[i] = *reinterpret_cast<const __nv_bfloat16*>(xh + place(i));
   }
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");

@@ -251,18 +251,14 @@ __device__ __forceinline__ void pack32(const float (&v)[32], uint4 (&o)[Slots<T>
   }
 }
 
-// A float32 value as a sum of three bf16 values (8 + 8 + 8 bits): the remainders are exact in fp32.  Where the first would
-// round up to infinity all are cut instead, so that no partial sum passes the value; infinities and NaN stay in the first
-// plane alone.
+// A float32 value as the exact sum of three bf16 values (8 + 8 + 8 bits), cut off towards zero, so that none passes the value.
+// Without branches: 32 of these run side by side.  Infinities stay in the first part alone.
+__device__ __forceinline__ float cut16(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 __device__ __forceinline__ void split3(float v, float& p0, float& p1, float& p2) {
-  p0 = __bfloat162float(__float2bfloat16_rn(v));
-  p1 = __bfloat162float(__float2bfloat16_rn(v - p0));
-  if (isinf(p0)) {
-    p0 = __bfloat162float(__float2bfloat16_rz(v));
-    p1 = __bfloat162float(__float2bfloat16_rz(v - p0));
-  }
-  p2 = v - p0 - p1;
-  if (!isfinite(v)) { p0 = v; p1 = 0.f; p2 = 0.f; }
+  p0 = cut16(v);
+  const float r = p0 == v ? 0.f : v - p0;
+  p1 = cut16(r);
+  p2 = r - p1;
 }
 
 // 32 columns of the sum of a group's accumulators, STRIDE columns apart.

@@ -8,11 +8,13 @@
 // g and u are formed again in the kernel that forms dh (three accumulators of one tile) instead of being kept: at the widths
 // of per-atom networks (K <= 1024) the extra 4 M K H operations cost less than writing and reading 2 M H values in 32 bits,
 // and 16-bit copies would add their rounding to every gradient.  What is rounded to 16 bits is what the next product reads:
-// h, dg and du, once each.
+// h, dg and du, once each.  Over many rows and columns those roundings average out (the error of a result is sqrt(2) times its
+// own rounding); up to 256 rows, where the products cost next to nothing, they are kept as a 16-bit value and a 16-bit
+// remainder and the next product reads both.
 //
 // float32 matrices run on the same tensor cores: a value is the exact sum of three bf16 values and a product the six
 // partial products down to 2^-24; the intermediate h, dg and du are stored as three planes each, so nothing is lost to
-// 16 bits.
+// 16 bits.  There dh is a product of its own (its accumulators would not fit beside those of g and u).
 #include "dense16.cuh"
 
 namespace nva {
@@ -40,21 +42,30 @@ __device__ __forceinline__ float fast_rcp(float x) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// act(g) and act'(g); EXACT: float32 results (library exponential and division), else the fast ones (1e-6 relative).
+// The same to fp32 accuracy, without branches.  e^x = 2^t e^(d ln 2) with t = x log2(e) rounded and d what the rounding left;
+// one Newton step for the reciprocal.
+__device__ __forceinline__ float exp32(float x) {
+  x = fminf(fmaxf(x, -87.f), 87.f);
+  const float t = x * kLog2e, d = fmaf(x, kLog2e, -t) + x * 1.925963033e-8f;  // log2(e) - kLog2e
+  return fast_exp2(t) * fmaf(d, 0.69314718f, 1.f);
+}
+__device__ __forceinline__ float rcp32(float x) {
+  const float r = fast_rcp(x);
+  return fmaf(r, fmaf(-x, r, 1.f), r);
+}
+
+// act(g) and act'(g); EXACT: for float32 results, else with the fast functions (1e-6 relative).
 template <bool EXACT, int ACT>
 __device__ __forceinline__ void activate(float g, float& a, float& da) {
   if constexpr (ACT == kSilu) {
-    const float s = EXACT ? 1.f / (1.f + expf(-g)) : fast_rcp(1.f + fast_exp2(-kLog2e * g));
+    const float e = EXACT ? exp32(-g) : fast_exp2(-kLog2e * g), s = EXACT ? rcp32(1.f + e) : fast_rcp(1.f + e);
     a = g * s;
     da = s * (1.f + g * (1.f - s));
-  } else if constexpr (EXACT) {  // g * Phi(g)
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-    a = g * cdf;
-    da = cdf + g * 0.39894228040143268f * expf(-0.5f * g * g);
-  } else {
+  } else {  // g * Phi(g)
     // erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), z >= 0: Hastings' approximation (Abramowitz and Stegun,
     // 7.1.26), off by at most 1.5e-7; its exponential is the derivative's as well
-    const float z = 0.70710678118654752f * fabsf(g), e = fast_exp2(-0.5f * kLog2e * g * g), t = fast_rcp(1.f + 0.3275911f * z);
+    const float z = 0.70710678118654752f * fabsf(g), q0 = 1.f + 0.3275911f * z;
+    const float e = EXACT ? exp32(-0.5f * g * g) : fast_exp2(-0.5f * kLog2e * g * g), t = EXACT ? rcp32(q0) : fast_rcp(q0);
     const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
     const float cdf = g < 0.f ? q : 1.f - q;
     a = g * cdf;
@@ -86,10 +97,10 @@ __device__ __forceinline__ void gate_grad(float (&g)[C], float (&u)[C], float (&
   }
 }
 
-// C columns (16 or 32) of a warp's 32 rows as T, or as three bf16 planes of a float32 value.
+// C columns of a warp's 32 rows as T (two: and the remainder as T), or as three bf16 planes of a float32 value.
 template <typename T, int C>
 __device__ __forceinline__ void store_cols(uint4* stage, float (&v)[C], void* dst, int64_t off, int64_t ld, int64_t plane, int rows_left,
-                                           int cols_left) {
+                                           int cols_left, int two) {
   auto put = [&](const float (&f)[C], auto tag, int64_t at) {
     using S = decltype(tag);
     uint4 o[C / 8];
@@ -101,6 +112,11 @@ __device__ __forceinline__ void store_cols(uint4* stage, float (&v)[C], void* ds
   };
   if constexpr (sizeof(T) == 2) {
     put(v, T{}, off);
+    if (two) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] -= widen(narrow<T>(v[j]));
+      put(v, T{}, off + plane);
+    }
   } else {
     float p1[C], p2[C];
 #pragma unroll
@@ -115,66 +131,89 @@ __device__ __forceinline__ void store_cols(uint4* stage, float (&v)[C], void* ds
   }
 }
 
-// C columns of the accumulator (of several, see acc_ld32).
-template <int C, int ACC, int STRIDE>
-__device__ __forceinline__ void acc_ld(uint32_t tm, float (&v)[C], int used) {
-  if constexpr (C == 32) {
-    acc_ld32<ACC, STRIDE>(tm, v, used);
-  } else {
-    static_assert(C == 16 && ACC == 1, "dense: 16 columns of one accumulator");
-    tmem_ld16(tm, v);
-  }
-}
-
 // Columns [0, BN/2) of the accumulator: g, [BN/2, BN): u, both of the same BN/2 columns of h.
 template <typename T, int BN>
 struct EpiGated : NoPrefetch {
   static constexpr int kAcc = sizeof(T) == 4 ? 512 / BN : 1, kStride = BN;
   static constexpr bool kLate = false;
-  struct Params { void* h; int64_t ld, plane; int act; };
+  struct Params { void* h; int64_t ld, plane; int act, two; };
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
-    constexpr int COLS = BN / 4, C = 32;
     const int used = used_acc<kAcc>(t, at, 0);
 #pragma unroll 1
-    for (int cb = 0; cb < COLS / C; ++cb) {
-      const int c = part * COLS + cb * C, n0 = at.n * (BN / 2) + c;
-      float g[C], u[C];
-      acc_ld<C, kAcc, kStride>(tm + c, g, used);
-      acc_ld<C, kAcc, kStride>(tm + BN / 2 + c, u, used);
+    for (int cb = 0; cb < BN / 128; ++cb) {
+      const int c = part * (BN / 4) + cb * 32, n0 = at.n * (BN / 2) + c;
+      float g[32], u[32];
+      acc_ld32<kAcc, kStride>(tm + c, g, used);
+      acc_ld32<kAcc, kStride>(tm + BN / 2 + c, u, used);
       if (p.act == kSilu) gate<sizeof(T) == 4, kSilu>(g, u);
       else gate<sizeof(T) == 4, kGelu>(g, u);
-      store_cols<T>(stage, g, p.h, (int64_t)row0 * p.ld + n0, p.ld, p.plane, t.M - row0, t.N - n0);
+      store_cols<T>(stage, g, p.h, (int64_t)row0 * p.ld + n0, p.ld, p.plane, t.M - row0, t.N - n0, p.two);
     }
   }
 };
 
-// Of HC columns of h: g in accumulator columns [0, HC), u in [HC, 2 HC), dh after those.  One accumulator each: 128 columns, dh in
-// turns in two places (see dense_kernel).  Two accumulators, for float32 sums of more than 512 terms: 64 columns.
-template <typename T, int ACC>
+struct GradOut { void *dg, *du, *h; int64_t ld, plane; int act, two; };
+template <typename T>
+__device__ __forceinline__ void store_grads(const GradOut& p, const Tiles& t, int row0, int n0, uint4* stage, float (&g)[32], float (&u)[32],
+                                            float (&d)[32]) {
+  if (p.act == kSilu) gate_grad<sizeof(T) == 4, kSilu>(g, u, d);
+  else gate_grad<sizeof(T) == 4, kGelu>(g, u, d);
+  const int64_t off = (int64_t)row0 * p.ld + n0;
+  store_cols<T>(stage, g, p.dg, off, p.ld, p.plane, t.M - row0, t.N - n0, p.two);
+  store_cols<T>(stage, d, p.du, off, p.ld, p.plane, t.M - row0, t.N - n0, p.two);
+  store_cols<T>(stage, u, p.h, off, p.ld, p.plane, t.M - row0, t.N - n0, p.two);
+}
+
+// 16 bits: of 128 columns of h, g in accumulator columns [0, 128), u in [128, 256), dh after those, in turns in two places (see
+// dense_kernel).
+template <typename T>
 struct EpiGatedGrad : NoPrefetch {
-  static constexpr int kHc = ACC == 2 ? 64 : 128;
-  static constexpr int kAcc = ACC, kStride = 192;
-  static constexpr bool kLate = ACC == 1;
-  struct Params { void *dg, *du, *h; int64_t ld, plane; int act; };
+  static constexpr int kAcc = 1, kStride = 0;
+  static constexpr bool kLate = true;
+  using Params = GradOut;
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
-    constexpr int COLS = kHc / 2, C = 32;
-    const int used = used_acc<kAcc>(t, at, 0), used1 = used_acc<kAcc>(t, at, 1);
-    const uint32_t td = tm + 2 * kHc + (kLate ? (at.seq & 1) * 128 : 0);
+    const uint32_t td = tm + 256 + (at.seq & 1) * 128;
 #pragma unroll 1
-    for (int cb = 0; cb < COLS / C; ++cb) {
-      const int c = part * COLS + cb * C, n0 = at.n * kHc + c;
-      float g[C], u[C], d[C];
-      acc_ld<C, kAcc, kStride>(tm + c, g, used);
-      acc_ld<C, kAcc, kStride>(tm + kHc + c, u, used);
-      acc_ld<C, kAcc, kStride>(td + c, d, used1);
-      if (p.act == kSilu) gate_grad<sizeof(T) == 4, kSilu>(g, u, d);
-      else gate_grad<sizeof(T) == 4, kGelu>(g, u, d);
-      const int64_t off = (int64_t)row0 * p.ld + n0;
-      store_cols<T>(stage, g, p.dg, off, p.ld, p.plane, t.M - row0, t.N - n0);
-      store_cols<T>(stage, d, p.du, off, p.ld, p.plane, t.M - row0, t.N - n0);
-      store_cols<T>(stage, u, p.h, off, p.ld, p.plane, t.M - row0, t.N - n0);
+    for (int cb = 0; cb < 2; ++cb) {
+      const int c = part * 64 + cb * 32;
+      float g[32], u[32], d[32];
+      tmem_ld32(tm + c, g);
+      tmem_ld32(tm + 128 + c, u);
+      tmem_ld32(td + c, d);
+      store_grads<T>(p, t, row0, at.n * 128 + c, stage, g, u, d);
+    }
+  }
+};
+
+// float32: g and u as in EpiGated, dh [M][ld_dh] (rows on 16-byte boundaries) from memory.
+template <int BN>
+struct EpiGatedGradRead {
+  static constexpr int kAcc = 512 / BN, kStride = BN;
+  static constexpr bool kLate = false;
+  struct Params { GradOut out; const float* dh; int64_t ld_dh; };
+  struct Pre { uint4 raw[8]; };  // 32 columns of dh
+  static __device__ __forceinline__ void fetch(const Params& p, const Tiles& t, int row0, int n0, Pre& pre) {
+    fetch_piece<float, 8>(pre.raw, p.dh + (int64_t)row0 * p.ld_dh + n0, p.ld_dh, t.M - row0, t.N - n0);
+  }
+  static __device__ __forceinline__ void prefetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int part, Pre& pre) {
+    fetch(p, t, row0, at.n * (BN / 2) + part * (BN / 4), pre);
+  }
+  static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
+                                             uint4* stage, Pre& pre) {
+    const int used = used_acc<kAcc>(t, at, 0);
+#pragma unroll 1
+    for (int cb = 0; cb < BN / 128; ++cb) {
+      const int c = part * (BN / 4) + cb * 32, n0 = at.n * (BN / 2) + c;
+      float g[32], u[32], d[32];
+      turn_piece<8>(stage, pre.raw);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) d[j] = reinterpret_cast<const float*>(pre.raw)[j];
+      if (cb + 1 < BN / 128) fetch(p, t, row0, n0 + 32, pre);
+      acc_ld32<kAcc, kStride>(tm + c, g, used);
+      acc_ld32<kAcc, kStride>(tm + BN / 2 + c, u, used);
+      store_grads<float>(p.out, t, row0, n0, stage, g, u, d);
     }
   }
 };
@@ -232,6 +271,7 @@ __global__ void split_sum_kernel(const float* __restrict__ partial, int splits, 
 struct Operand {
   Stored s;
   Tensor keep, source;
+  int planes = 1;  // parts of a value: 1, 2 (16-bit value and remainder) or 3 (float32)
   bool rowmajor = true;
   bool mn(int k_axis) const { return rowmajor != (k_axis == 1); }
   int64_t extent(int axis) const { return (axis == 1) == rowmajor ? s.inner : s.outer; }
@@ -254,7 +294,7 @@ Operand operand(Tensor t, PackJobs& jobs, bool rowmajor) {
     o.s = {t.data_ptr(), cols, rows, ld, 1, 0};
     return o;
   }
-  const int P = planes_of(t);
+  const int P = o.planes = planes_of(t);
   const int64_t ldp = (cols + 7) / 8 * 8;
   o.source = t;
   o.keep = at::empty({P, rows, ldp}, t.options().dtype(P == 3 ? at::kBFloat16 : t.scalar_type()));
@@ -266,42 +306,51 @@ Operand operand(Tensor t, PackJobs& jobs, bool rowmajor) {
 Operand operand(const Tensor& t, PackJobs& jobs) { return operand(t, jobs, by_rows(t)); }
 
 // Intermediate [P][rows][ld] (16-bit) that epilogues write and later products read.
-Operand intermediate(int64_t rows, int64_t cols, int P, const Tensor& like, int copies = 1) {
+Operand intermediate(int64_t rows, int64_t cols, int planes, const Tensor& like, int copies = 1) {
   Operand o;
   const int64_t ld = (cols + 7) / 8 * 8;
-  o.keep = at::empty({copies * P, rows, ld}, like.options().dtype(P == 3 ? at::kBFloat16 : like.scalar_type()));
-  o.s = {o.keep.data_ptr(), cols, rows, ld, copies * P, rows * ld};
+  o.planes = planes;
+  o.keep = at::empty({copies * planes, rows, ld}, like.options().dtype(like.scalar_type() == at::kFloat ? at::kBFloat16 : like.scalar_type()));
+  o.s = {o.keep.data_ptr(), cols, rows, ld, copies * planes, rows * ld};
   return o;
 }
 
 struct Plan {
   Maps maps;
   Tiles t{};
-  int n_maps = 0, P;
+  int n_maps = 0;
   bool bf16;
-  Plan(int P_, bool bf16_) : P(P_), bf16(bf16_) {}
+  explicit Plan(bool bf16_) : bf16(bf16_) {}
   int map(const Operand& o) { put_map(maps, n_maps, o.s); return n_maps++; }
   // a[.., k] . b[.., k]; ka / kb: the axis of each logical matrix that is contracted; b2 < 0: both halves from b.
-  // part 0: the small partial products of float32 operands (added first), 1: the large one, 2: both.
+  // part 0: the small partial products (added first), 1: the large one, 2: both.
   void product(int a, const Operand& oa, int ka, int b, int b2, const Operand& ob, int kb, int col, int n, int a_z = 0, int b_z = 0,
                int a_step = 0, int b_step = 0, int part = 2, int group = 0) {
     const int64_t K = oa.extent(ka);
-    static const int order[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};  // what is left out is below 2^-24
-    for (int i = P == 3 && part != 1 ? 0 : 5; i < (part == 0 ? (P == 3 ? 5 : 0) : 6); ++i) {
+    auto add = [&](int za, int zb) {
+      const bool main = za + zb == 0;
+      if (part != 2 && main != (part == 1)) return;
       TORCH_CHECK(t.n_seg < kMaxSegs, "dense: too many segments");
       Seg& s = t.seg[t.n_seg++];
       s.a = (int8_t)a; s.b = (int8_t)b; s.b2 = (int8_t)(b2 < 0 ? b : b2);
       s.a_mn = oa.mn(ka); s.b_mn = ob.mn(kb);
       s.group = (int8_t)group;
-      s.spread = i == 5;
+      s.spread = main;
       s.col = (int16_t)col; s.n = (int16_t)n;
-      s.za = a_z + order[i][0]; s.zb = b_z + order[i][1];
+      s.za = a_z + za; s.zb = b_z + zb;
       s.za_step = a_step; s.zb_step = b_step;
       s.nk = (int)((K + BK - 1) / BK);
       s.b2_off = b2 < 0 ? n / 2 : 0;
       s.idesc = idesc16(bf16, s.a_mn, s.b_mn, n, BM);
-      if (s.spread) t.main_nk[group] = s.nk;
+      if (main) t.main_nk[group] = s.nk;
+    };
+    if (oa.planes == 3 && ob.planes == 3) {  // what is left out is below 2^-24
+      add(2, 0); add(0, 2); add(1, 1); add(1, 0); add(0, 1);
+    } else {
+      if (oa.planes == 2) add(1, 0);
+      if (ob.planes == 2) add(0, 1);
     }
+    add(0, 0);
   }
 };
 
@@ -312,9 +361,11 @@ template <typename T, int BN, int ACC>
 void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   set_tiles(pl.t, M, N, BN, batches, 1);
   const int tiles = pl.t.total, nk = pl.t.main_nk[0], kb = nk * pl.t.n_seg, at_once = slots(pl.t);
+  int mains = 0;  // large partial products that add to the same accumulators
+  for (int i = 0; i < pl.t.n_seg; ++i) mains += pl.t.seg[i].spread;
   int splits = 1;
   if (2 * tiles <= at_once) splits = std::max(1, std::min({at_once / tiles, kb / 8, nk, 64}));
-  if (ACC > 1) splits = std::max(splits, (nk + 8 * ACC - 1) / (8 * ACC));
+  if (ACC > 1) splits = std::min(nk, std::max(splits, (nk * mains + 8 * ACC - 1) / (8 * ACC)));
   if (splits == 1) {
     typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
     run_dense<BN, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);
@@ -337,6 +388,8 @@ int store_bn(int64_t batches, int64_t M, int64_t N, int64_t kb) {
   if (wide < pairs && 4 * wide * std::min(pairs / wide, kb / 8) >= 3 * pairs) return 256;
   return pick_bn(wide, rows * ((N + 127) / 128));
 }
+// Parts in which intermediates are kept: 16-bit ones of few rows with their remainder.
+int parts_of(int P, int64_t M) { return P == 1 && M <= 256 ? 2 : P; }
 // Blocks of the contraction axis of a product with an axis of K.
 int64_t blocks_of(int P, int64_t K) { return (K + BK - 1) / BK * (P == 3 ? 6 : 1); }
 void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
@@ -386,16 +439,17 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
   PackJobs jobs;
   Operand ox = operand(x, jobs), og = operand(wg, jobs), ou = operand(wu, jobs, og.rowmajor), od = operand(wd, jobs);
   run_packs(jobs, P, st);
-  Operand oh = intermediate(M, H, P, x);
+  const int Pi = parts_of(P, M);
+  Operand oh = intermediate(M, H, Pi, x);
   {
-    Plan pl(P, bf16);
+    Plan pl(bf16);
     const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou);
     auto go = [&](auto v, auto bn_tag) {
       using T = decltype(v);
       constexpr int BN = decltype(bn_tag)::value;
       pl.product(a, ox, 1, b, b2, og, 0, 0, BN);
       set_tiles(pl.t, M, H, BN / 2, 1, 1);
-      typename EpiGated<T, BN>::Params ep{oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act};
+      typename EpiGated<T, BN>::Params ep{oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act, Pi == 2 ? 1 : 0};
       run_dense<BN, EpiGated<T, BN>>(pl.maps, pl.t, ep, st);
     };
     auto wide = [&](auto v) {
@@ -406,7 +460,7 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
     else if (bf16) wide(__nv_bfloat16{});
     else wide(__half{});
   }
-  Plan pl(P, bf16);
+  Plan pl(bf16);
   const int bn = store_bn(1, M, N, blocks_of(P, H));
   const int a = pl.map(oh), b = pl.map(od);
   pl.product(a, oh, 1, b, -1, od, 0, 0, bn);
@@ -436,48 +490,58 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
   PackJobs jobs;
   Operand ox = operand(x, jobs), og = operand(wg, jobs), ou = operand(wu, jobs, og.rowmajor), od = operand(wd, jobs), oy = operand(dy, jobs);
   run_packs(jobs, P, st);
-  Operand oe = intermediate(M, H, P, x, 2), oh = intermediate(M, H, P, x);  // dg then du; h
-  {
-    Plan pl(P, bf16);
+  const int Pi = parts_of(P, M);
+  Operand oe = intermediate(M, H, Pi, x, 2), oh = intermediate(M, H, Pi, x);  // dg then du; h
+  uint16_t* const e = (uint16_t*)oe.keep.data_ptr();
+  const GradOut out{e, e + Pi * oe.s.plane, oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act, Pi == 2 ? 1 : 0};
+  if (P == 1) {
+    Plan pl(bf16);
     const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou), a3 = pl.map(oy), b3 = pl.map(od);
-    const bool deep = P == 3 && std::max(K, N) > 512;
-    const int hc = deep ? 64 : 128;
-    for (int part = 0; part < 2; ++part) pl.product(a3, oy, 1, b3, -1, od, 1, 2 * hc, hc, 0, 0, 0, 0, part, 1);
-    for (int part = 0; part < 2; ++part) pl.product(a, ox, 1, b, b2, og, 0, 0, 2 * hc, 0, 0, 0, 0, part);
-    set_tiles(pl.t, M, H, hc, 1, 1, false, !deep);  // 64 columns of dh are too few for a pair
-    auto go = [&](auto v, auto acc) {
-      using T = decltype(v);
-      constexpr int ACC = decltype(acc)::value;
-      using Epi = EpiGatedGrad<T, ACC>;
-      uint16_t* e = (uint16_t*)oe.keep.data_ptr();
-      typename Epi::Params ep{e, e + P * oe.s.plane, oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act};
-      run_dense<2 * Epi::kHc, Epi, ACC == 1>(pl.maps, pl.t, ep, st);
+    pl.product(a3, oy, 1, b3, -1, od, 1, 256, 128, 0, 0, 0, 0, 2, 1);
+    pl.product(a, ox, 1, b, b2, og, 0, 0, 256);
+    set_tiles(pl.t, M, H, 128, 1, 1);
+    if (bf16) run_dense<256, EpiGatedGrad<__nv_bfloat16>>(pl.maps, pl.t, out, st);
+    else run_dense<256, EpiGatedGrad<__half>>(pl.maps, pl.t, out, st);
+  } else {
+    const int64_t ld_dh = (H + 3) / 4 * 4;  // columns past H come out as zeros
+    Tensor dh = at::empty({M, ld_dh}, x.options());
+    {
+      Plan pl(bf16);
+      const int bn = store_bn(1, M, ld_dh, blocks_of(P, N));
+      const int a = pl.map(oy), b = pl.map(od);
+      pl.product(a, oy, 1, b, -1, od, 1, 0, bn);
+      store_any(pl, bn, dh, 1, M, ld_dh, st);
+    }
+    Plan pl(bf16);
+    const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou);
+    auto go = [&](auto bn_tag) {
+      constexpr int BN = decltype(bn_tag)::value;
+      pl.product(a, ox, 1, b, b2, og, 0, 0, BN);
+      set_tiles(pl.t, M, H, BN / 2, 1, 1);
+      run_dense<BN, EpiGatedGradRead<BN>>(pl.maps, pl.t, {out, dh.data_ptr<float>(), ld_dh}, st);
     };
-    using One = std::integral_constant<int, 1>;
-    if (deep) go(float{}, std::integral_constant<int, 2>{});
-    else if (P == 3) go(float{}, One{});
-    else if (bf16) go(__nv_bfloat16{}, One{});
-    else go(__half{}, One{});
+    if (store_bn(1, M, 2 * H, 0) == 256) go(std::integral_constant<int, 256>{});
+    else go(std::integral_constant<int, 128>{});
   }
   if (which & 1) {
-    Plan pl(P, bf16);
+    Plan pl(bf16);
     const int bn = store_bn(1, M, K, 2 * blocks_of(P, H));
     const int a = pl.map(oe), b = pl.map(og), c = pl.map(ou);
     for (int part = 0; part < 2; ++part) {
       pl.product(a, oe, 1, b, -1, og, 1, 0, bn, 0, 0, 0, 0, part);
-      pl.product(a, oe, 1, c, -1, ou, 1, 0, bn, P, 0, 0, 0, part);
+      pl.product(a, oe, 1, c, -1, ou, 1, 0, bn, Pi, 0, 0, 0, part);
     }
     store_any(pl, bn, dx, 1, M, K, st);
   }
   if (which & 2) {
-    Plan pl(P, bf16);
+    Plan pl(bf16);
     const int bn = store_bn(2, K, H, blocks_of(P, M));
     const int a = pl.map(ox), b = pl.map(oe);
-    pl.product(a, ox, 0, b, -1, oe, 0, 0, bn, 0, 0, 0, P);
+    pl.product(a, ox, 0, b, -1, oe, 0, 0, bn, 0, 0, 0, Pi);
     store_any(pl, bn, dgu, 2, K, H, st);
   }
   if (which & 4) {
-    Plan pl(P, bf16);
+    Plan pl(bf16);
     const int bn = store_bn(1, H, N, blocks_of(P, M));
     const int a = pl.map(oh), b = pl.map(oy);
     pl.product(a, oh, 0, b, -1, oy, 0, 0, bn);

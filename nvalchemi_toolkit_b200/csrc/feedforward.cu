@@ -356,7 +356,7 @@ struct Plan {
 
 // Plain product into `out` [batches][M][N].  The contraction axis is split over several tiles (partials added in order by a
 // second kernel) when half of the GPU or more would have no tile and the axis is long, and for float32 so that no accumulator
-// takes more than 32 instructions of the large partial product.
+// takes more than 32 instructions of the large partial product (up to 64 partials: 131,072 terms in sums of 64 instructions).
 template <typename T, int BN, int ACC>
 void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   set_tiles(pl.t, M, N, BN, batches, 1);
@@ -365,7 +365,7 @@ void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N,
   for (int i = 0; i < pl.t.n_seg; ++i) mains += pl.t.seg[i].spread;
   int splits = 1;
   if (2 * tiles <= at_once) splits = std::max(1, std::min({at_once / tiles, kb / 8, nk, 64}));
-  if (ACC > 1) splits = std::min(nk, std::max(splits, (nk * mains + 8 * ACC - 1) / (8 * ACC)));
+  if (ACC > 1) splits = std::min({nk, 64, std::max(splits, (nk * mains + 8 * ACC - 1) / (8 * ACC))});
   if (splits == 1) {
     typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
     run_dense<BN, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);

@@ -19,6 +19,7 @@ from nvalchemi_toolkit_b200.ops._native_counter import ops as _nops
 COEFFICIENTS = (3.4445, -4.775, 2.0315)
 #: Bound of the iterate's singular values for which the float16 operands (X and A times 2^12, B times 2^11) cannot overflow.
 _MAX_VALUE = 2.5
+_MAX_BATCH = 65535  # matrices of one launch
 
 
 def _check(g: torch.Tensor, steps: int, coefficients: tuple[float, float, float], eps: float) -> None:
@@ -60,8 +61,10 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: tuple[float, fl
         if not g.is_cuda:
             return _formula(g.detach().float(), int(steps), a, b, c, float(eps)).to(torch.bfloat16)
         _native.require(g)
-        out = _nops.newton_schulz(g.reshape(math.prod(g.shape[:-2]), *g.shape[-2:]).contiguous(), int(steps), a, b, c, float(eps))
-        return out.view(g.shape)
+        batch = g.reshape(math.prod(g.shape[:-2]), *g.shape[-2:]).contiguous()
+        parts = batch.split(_MAX_BATCH) if batch.shape[0] > _MAX_BATCH else (batch,)
+        outs = [_nops.newton_schulz(p, int(steps), a, b, c, float(eps)) for p in parts]
+        return (outs[0] if len(outs) == 1 else torch.cat(outs)).view(g.shape)
 
 
 def _formula(x: torch.Tensor, steps: int, a: float, b: float, c: float, eps: float) -> torch.Tensor:

@@ -117,6 +117,35 @@ def test_layouts(m, k, h, n, dtype, layout):
     _run(m, k, h, n, dtype, "cuda", layout=layout)
 
 
+def test_one_row_without_a_batch_axis_and_more_axes(device):
+    x, wg, wu, wd, dy = _inputs(6, 16, 24, 8, F32, device)
+    y = ff.gated_feed_forward(x, wg, wu, wd)
+    dx, *_ = ff.gated_feed_forward_backward(dy, x, wg, wu, wd)
+    one = ff.gated_feed_forward(x[2], wg, wu, wd)
+    assert one.shape == (8,) and float((one - y[2]).abs().max()) < 64 * 2.0 ** -23 * float(y.abs().max())
+    deep = ff.gated_feed_forward(x.view(3, 1, 2, 16), wg, wu, wd)
+    assert deep.shape == (3, 1, 2, 8) and torch.equal(deep.view(6, 8), y)
+    again, *_ = ff.gated_feed_forward_backward(dy.view(3, 2, 8), x.view(3, 2, 16), wg, wu, wd)
+    assert again.shape == (3, 2, 16) and torch.equal(again.view(6, 16), dx)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls on two streams share nothing: each gives what it gives alone."""
+    a, b = _inputs(700, 96, 160, 96, BF16, "cuda"), _inputs(500, 64, 256, 64, F32, "cuda")
+    want = [[ff.gated_feed_forward(*t[:4]), *ff.gated_feed_forward_backward(t[4], *t[:4])] for t in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, t in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i] = [ff.gated_feed_forward(*t[:4]), *ff.gated_feed_forward_backward(t[4], *t[:4])]
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for x, y in zip(want, got) for p, q in zip(x, y))
+    assert ff.check_errors(a[0]) == 0
+
+
 @pytest.mark.gpu
 def test_same_bits_again_and_rows_do_not_mix():
     a = _run(500, 128, 384, 128, BF16, "cuda")

@@ -113,6 +113,15 @@ def test_shapes(device, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(65537, 2, 3), (65536, 1, 260)])
+def test_more_matrices_than_one_launch_takes(shape):
+    g = torch.randn(shape, device="cuda")
+    o = ortho.newton_schulz(g)
+    assert torch.equal(o[-3:], ortho.newton_schulz(g[-3:])) and torch.equal(o[:3], ortho.newton_schulz(g[:3]))
+    assert bool(o.isfinite().all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(6, 96, 128), (1, 400, 260)])
 def test_captured_and_repeated(shape):
     g = torch.randn(shape, device="cuda")

@@ -216,7 +216,9 @@ void product(const X* x, int64_t ldx, int64_t sx, const Weight& a, const Weight&
     else go(rows_by_n_kernel<T, X, 1, MATS, R>, (n + 7) / 8, 1);
     return;
   }
-  // blocks of a cluster: enough for two blocks on every SM, as long as each still has 64 rows of the weights
+  // blocks of a cluster: enough for two blocks on every SM, as long as each still has 64 rows of the weights (1024 -> 4096 -> 1024,
+  // one row, both launches: 50 us without clusters, 27 us in twos, 16.7 us in fours, 16.3 us in eights; with eight loads in
+  // flight a thread instead of four 18.3 us; the cluster barriers are 1.8 us of a launch)
   auto split = [&](int blocks) {
     int parts = 1;
     while (parts < 8 && blocks * parts < 296 && k / (2 * parts) >= 64) parts *= 2;

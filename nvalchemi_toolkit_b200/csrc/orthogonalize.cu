@@ -18,7 +18,12 @@
 // 128 or less fewer roundings average out (up to 3e-3 at 8 x 8), while the products cost little: there the remainder takes part
 // in A (three products) and in B X (two), which brings the error under 1e-3.
 //
-// A and B are symmetric: only tiles on and below the diagonal are computed, each is written twice.
+// A and B are symmetric: where the GPU has no tile to spare only those on and below the diagonal are computed, each written
+// twice.
+//
+// What bounds it: 4 x 1024 x 4096 bfloat16 takes 566 us: a step is 32 us for A (540 TFLOP/s of what has to be computed; 128-wide
+// tiles, 144 of them), 18 us for B (one short product and its epilogue) and 57 us for the update (600 TFLOP/s; its epilogue reads
+// and writes X, 270 MB a step in all).  Small problems are bound by latency: 1537 x 515 takes 17 launches of 9 to 14 us.
 #include "dense16.cuh"
 
 namespace nva {

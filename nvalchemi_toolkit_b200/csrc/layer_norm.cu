@@ -10,9 +10,9 @@
 // rows: float64); only the stored results are rounded to the tensors' types.
 // What counts is bytes under way: 64 bytes a thread (R rows of a group at a time where rows are short) and many resident
 // threads; loading the next rows ahead of a persistent block's reductions costs registers and with them residency, and was
-// slower (16,384 x 4096 float16 backward 182 us against 112 us).  In the backward pass the grid is persistent, a thread owns the same columns in every row it visits and keeps their dw / db sums in
-// registers; a block's row groups are added in a fixed order in shared memory, one partial row per block goes to the
-// workspace, and a second kernel adds the partial rows in a fixed order, so results do not change from run to run.
+// slower (16,384 x 4096 float16 backward 182 us against 112 us).  In the backward pass the grid is persistent, a thread owns the
+// same columns in every row it visits and keeps their dw / db sums in registers; a block's row groups are added in a fixed
+// order in shared memory, one partial row per block goes to the workspace, and a second kernel adds the partial rows in a fixed order, so results do not change from run to run.
 // 131,072 x 128 bfloat16: forward 18 us (3.7 TB/s), backward 27 us (3.7 TB/s) and 4 us for the sums; 16,384 x 4096 float16: 58 us
 // (4.6 TB/s), 100 us (4.0 TB/s) and 7 us.
 #include "common.cuh"

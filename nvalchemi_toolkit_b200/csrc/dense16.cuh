@@ -572,6 +572,25 @@ inline int pick_bn(int64_t tiles256, int64_t tiles128) {
 // Tiles that run at the same time.
 inline int slots(const Tiles& t) { return t.bm == BM ? sm_count() : sm_count() / 2; }
 
+// The small kernels of a chain take part in the early launches too: they call chain_wait() before they touch memory.
+__device__ __forceinline__ void chain_wait() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... P, typename... A>
+void launch_chained(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+
 template <int BN, bool PAIR, typename Epi>
 void launch_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cudaStream_t st) {
   constexpr int smem = smem_bytes<BN, PAIR>();

@@ -232,6 +232,7 @@ struct PackJobs { PackJob j[kMaxPacks]; int n = 0; };
 
 template <typename T, int P>
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
+  chain_wait();
   const PackJob job = jobs.j[blockIdx.y];
   const int64_t half = (job.cols + 1) / 2, total = job.rows * half;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
@@ -257,14 +258,13 @@ void run_packs(const PackJobs& jobs, int planes, cudaStream_t st) {
   int64_t most = 0;
   for (int i = 0; i < jobs.n; ++i) most = std::max(most, jobs.j[i].rows * ((jobs.j[i].cols + 1) / 2));
   const dim3 grid((unsigned)std::min<int64_t>((most + 255) / 256, 148 * 8), (unsigned)jobs.n);
-  if (planes == 3) pack_kernel<float, 3><<<grid, 256, 0, st>>>(jobs);
-  else pack_kernel<__half, 1><<<grid, 256, 0, st>>>(jobs);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_chained(planes == 3 ? pack_kernel<float, 3> : pack_kernel<__half, 1>, grid, 256, st, jobs);
 }
 
 // out = sum over splits of partial [splits][n], in order.
 template <typename T>
 __global__ void split_sum_kernel(const float* __restrict__ partial, int splits, int64_t stride, int64_t n, T* __restrict__ out) {
+  chain_wait();
   const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
   if (i >= n) return;
   float s = 0.f;
@@ -382,8 +382,7 @@ void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N,
   Tensor part = at::empty({splits, n}, out.options().dtype(at::kFloat));
   typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n, 1.f};
   run_dense<BN, EpiStore<float, BN, ACC>>(pl.maps, pl.t, ep, st);
-  split_sum_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(part.data_ptr<float>(), splits, n, n, (T*)out.data_ptr());
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  launch_chained(split_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), 256, st, part.data_ptr<float>(), splits, n, n, (T*)out.data_ptr());
 }
 
 // Columns of a tile of an M x N product over `kb` blocks of the contraction axis (all segments): by the number of tiles, and 256

@@ -210,6 +210,7 @@ __device__ __forceinline__ void load8(const T* p, bool vec, int left, double (&v
 // Sums of squares of G in float64 (no gradient is too small or too large for them): one partial per block.
 template <typename T>
 __global__ void __launch_bounds__(256) ns_norm_kernel(const T* __restrict__ g, int64_t count, bool vec, double* __restrict__ partial) {
+  chain_wait();
   const T* src = g + blockIdx.y * count;
   double s = 0.0;
   for (int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) * 8; i < count; i += (int64_t)gridDim.x * blockDim.x * 8) {
@@ -234,6 +235,7 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const T* __restrict__ g, i
                                                       const double* __restrict__ partial, int parts, double eps, __half* __restrict__ x,
                                                       int64_t plane) {
   __shared__ double scale;
+  chain_wait();
   if (threadIdx.x < 32) {
     double s = 0.0;
     for (int i = threadIdx.x; i < parts; i += 32) s += partial[blockIdx.y * parts + i];
@@ -539,8 +541,9 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
     using T = decltype(v);
     const T* p = (const T*)g.data_ptr();
     const bool vec = n % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
-    ns_norm_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(p, m * n, vec, partial.data_ptr<double>());
-    ns_init_kernel<T><<<dim3(parts, batch), 256, 0, st>>>(p, (int)m, (int)n, (int)ld, vec, partial.data_ptr<double>(), parts, eps, x0, plane);
+    launch_chained(ns_norm_kernel<T>, dim3(parts, batch), 256, st, p, m * n, vec, partial.data_ptr<double>());
+    launch_chained(ns_init_kernel<T>, dim3(parts, batch), 256, st, p, (int)m, (int)n, (int)ld, vec, partial.data_ptr<double>(), parts, eps, x0,
+                   plane);
   };
   if (g.scalar_type() == at::kFloat) prep(float{});
   else if (g.scalar_type() == at::kHalf) prep(__half{});

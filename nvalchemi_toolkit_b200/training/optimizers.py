@@ -86,7 +86,7 @@ class Muon(torch.optim.Optimizer):
         from nvalchemi_toolkit_b200.ops.orthogonalize import newton_schulz
 
         grads = [p.grad for p in ps]
-        bufs = [self.state[p].setdefault("momentum_buffer", torch.zeros_like(p, memory_format=torch.preserve_format)) for p in ps]
+        bufs = [self._buffer(p, "momentum_buffer") for p in ps]
         torch._foreach_mul_(bufs, group["momentum"])
         torch._foreach_add_(bufs, grads)
         updates = torch._foreach_add(grads, bufs, alpha=group["momentum"]) if group["nesterov"] else bufs
@@ -103,20 +103,23 @@ class Muon(torch.optim.Optimizer):
             p.add_(o[row: row + count].reshape(p.shape).to(p.dtype), alpha=-group["lr"] * scale)
             row += count
 
-    def _adam_step(self, p: torch.Tensor, group: dict[str, Any]) -> None:
+    def _buffer(self, p: torch.Tensor, name: str) -> torch.Tensor:
+        """The state tensor ``name`` of ``p``, zeros when it is first asked for."""
         st = self.state[p]
-        if "exp_avg" not in st:
-            st["adam_step"] = 0
-            st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+        if name not in st:
+            st[name] = torch.zeros_like(p, memory_format=torch.preserve_format)
+        return st[name]
+
+    def _adam_step(self, p: torch.Tensor, group: dict[str, Any]) -> None:
+        avg, avg_sq = self._buffer(p, "exp_avg"), self._buffer(p, "exp_avg_sq")
         b1, b2 = group["betas"]
-        st["adam_step"] += 1
-        st["exp_avg"].lerp_(p.grad, 1 - b1)
-        st["exp_avg_sq"].mul_(b2).addcmul_(p.grad, p.grad, value=1 - b2)
-        denom = (st["exp_avg_sq"] / (1 - b2 ** st["adam_step"])).sqrt_().add_(group["adam_eps"])
+        step = self.state[p]["adam_step"] = self.state[p].get("adam_step", 0) + 1
+        avg.lerp_(p.grad, 1 - b1)
+        avg_sq.mul_(b2).addcmul_(p.grad, p.grad, value=1 - b2)
+        denom = (avg_sq / (1 - b2 ** step)).sqrt_().add_(group["adam_eps"])
         if group["weight_decay"]:
             p.mul_(1.0 - group["lr"] * group["weight_decay"])
-        p.addcdiv_(st["exp_avg"], denom, value=-group["lr"] / (1 - b1 ** st["adam_step"]))
+        p.addcdiv_(avg, denom, value=-group["lr"] / (1 - b1 ** step))
 
 
 class ParamGroupSpec(BaseModel):

@@ -28,6 +28,12 @@ def check_kwargs(cls: Any, kwargs: Mapping[str, Any], label: str) -> None:
         raise ValueError(f"{label} {getattr(cls, '__name__', cls)} does not accept {unknown}; accepted: {accepted}")
 
 
+def _state_type(p: torch.Tensor) -> torch.dtype:
+    """Type of a parameter's optimiser state: 16 bits are too few for running means (a mean of squares stops decaying in bfloat16
+    and vanishes in float16)."""
+    return torch.float32 if p.dtype in (torch.bfloat16, torch.float16) else p.dtype
+
+
 class Muon(torch.optim.Optimizer):
     """Momentum whose matrix updates are orthogonalised by Newton-Schulz products (``ops.orthogonalize.newton_schulz``).
 
@@ -40,7 +46,8 @@ class Muon(torch.optim.Optimizer):
     The factor gives an update of the root mean square size of an AdamW step, so ``lr`` and ``weight_decay`` are AdamW's.
     Parameters with fewer axes, matrices with a side of one, and groups with ``orthogonalize=False`` (embedding tables, for
     instance, by a ``ParamGroupSpec``) take AdamW steps with ``betas`` and ``adam_eps``.  Matrices of one shape are
-    orthogonalised together, one call for all of them."""
+    orthogonalised together, one call for all of them.  The state of 16-bit parameters is float32, their steps are formed in float32
+    and rounded once."""
 
     def __init__(self, params: Any, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  ns_steps: int = 5, betas: tuple[float, float] = (0.9, 0.999), adam_eps: float = 1e-8, orthogonalize: bool = True) -> None:
@@ -85,7 +92,7 @@ class Muon(torch.optim.Optimizer):
     def _matrix_step(self, ps: list[torch.Tensor], shape: tuple[int, int], group: dict[str, Any]) -> None:
         from nvalchemi_toolkit_b200.ops.orthogonalize import newton_schulz
 
-        grads = [p.grad for p in ps]
+        grads = [p.grad.to(_state_type(p)) for p in ps]
         bufs = [self._buffer(p, "momentum_buffer") for p in ps]
         torch._foreach_mul_(bufs, group["momentum"])
         torch._foreach_add_(bufs, grads)
@@ -95,31 +102,46 @@ class Muon(torch.optim.Optimizer):
             stacked = stacked.float()
         o = newton_schulz(stacked, steps=group["ns_steps"])
         scale = 0.2 * max(shape) ** 0.5
+        wide = [p.to(_state_type(p)) for p in ps]  # the parameters themselves, unless they have 16 bits
         if group["weight_decay"]:
-            torch._foreach_mul_(ps, 1.0 - group["lr"] * group["weight_decay"])
+            torch._foreach_mul_(wide, 1.0 - group["lr"] * group["weight_decay"])
         row = 0
-        for p in ps:
+        for p, w in zip(ps, wide):
             count = p.numel() // (shape[0] * shape[1])
-            p.add_(o[row: row + count].reshape(p.shape).to(p.dtype), alpha=-group["lr"] * scale)
+            w.add_(o[row: row + count].reshape(p.shape).to(w.dtype), alpha=-group["lr"] * scale)
             row += count
+            if w.dtype != p.dtype:
+                p.copy_(w)
 
     def _buffer(self, p: torch.Tensor, name: str) -> torch.Tensor:
         """The state tensor ``name`` of ``p``, zeros when it is first asked for."""
         st = self.state[p]
         if name not in st:
-            st[name] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            st[name] = torch.zeros_like(p, dtype=_state_type(p), memory_format=torch.preserve_format)
         return st[name]
+
+    def load_state_dict(self, state_dict: dict[str, Any]) -> None:
+        super().load_state_dict(state_dict)  # casts the state to the types of the parameters
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            if _state_type(p) != p.dtype:
+                for name, v in state_dict["state"].get(i, {}).items():
+                    if isinstance(v, torch.Tensor):
+                        self.state[p][name] = v.to(p.device, _state_type(p))
 
     def _adam_step(self, p: torch.Tensor, group: dict[str, Any]) -> None:
         avg, avg_sq = self._buffer(p, "exp_avg"), self._buffer(p, "exp_avg_sq")
         b1, b2 = group["betas"]
         step = self.state[p]["adam_step"] = self.state[p].get("adam_step", 0) + 1
-        avg.lerp_(p.grad, 1 - b1)
-        avg_sq.mul_(b2).addcmul_(p.grad, p.grad, value=1 - b2)
+        w, grad = p.to(avg.dtype), p.grad.to(avg.dtype)  # p itself, unless it has 16 bits
+        avg.lerp_(grad, 1 - b1)
+        avg_sq.mul_(b2).addcmul_(grad, grad, value=1 - b2)
         denom = (avg_sq / (1 - b2 ** step)).sqrt_().add_(group["adam_eps"])
         if group["weight_decay"]:
-            p.mul_(1.0 - group["lr"] * group["weight_decay"])
-        p.addcdiv_(avg, denom, value=-group["lr"] / (1 - b1 ** step))
+            w.mul_(1.0 - group["lr"] * group["weight_decay"])
+        w.addcdiv_(avg, denom, value=-group["lr"] / (1 - b1 ** step))
+        if w.dtype != p.dtype:
+            p.copy_(w)
 
 
 class ParamGroupSpec(BaseModel):

@@ -26,8 +26,9 @@
 // the instructions need 320 ns; an instruction of 128 or 64 columns needs 195 ns whichever it is.  A pair writes 32 KB and reads
 // 32 KB per CTA.
 //
-// Every wait is bounded; on expiry the error word is set, the roles leave their loops, the producer waits (bounded) for its
-// copies in flight, and the TMEM is freed.
+// Every wait is bounded; on expiry the error word is set, the products stop, the producer waits (bounded) for its copies in
+// flight, the epilogue goes on with NaN in the place of the accumulators (no finite result is left that nothing has formed), and
+// the TMEM is freed.
 #pragma once
 #include "common.cuh"
 #include "convert.cuh"
@@ -72,7 +73,10 @@ struct Tiles {
 
 struct alignas(64) Maps { CUtensorMap m[kMaxMaps]; int n = 0; };
 
-struct TileAt { int m, n, batch, split, seq; };  // seq: the CTA's how-manieth tile
+struct TileAt {
+  int m, n, batch, split, seq;  // seq: the CTA's how-manieth tile
+  bool ok;                      // its products are done; false after an expired wait, the same for all lanes of a warp
+};
 
 // The part of a segment's blocks that one of `splits` tiles of the same output takes.
 __device__ __forceinline__ int split_at(int nk, int split, int splits) {
@@ -90,6 +94,7 @@ __device__ __forceinline__ int used_acc(const Tiles& t, const TileAt& at, int gr
 __device__ __forceinline__ TileAt tile_at(const Tiles& t, int i, int seq) {
   TileAt r;
   r.seq = seq;
+  r.ok = true;
   const int per = t.lower ? t.lower * (t.mt * (t.mt + 1) / 2) : t.mt * t.nt;
   const int z = i / per;
   const int j = i - z * per;
@@ -261,9 +266,14 @@ __device__ __forceinline__ void split3(float v, float& p0, float& p1, float& p2)
   p2 = r - p1;
 }
 
-// 32 columns of the sum of a group's accumulators, STRIDE columns apart.
+// 32 columns of the sum of a group's accumulators, STRIDE columns apart; NaN after an expired wait.
 template <int ACC, int STRIDE>
-__device__ __forceinline__ void acc_ld32(uint32_t tm, float (&v)[32], int used) {
+__device__ __forceinline__ void acc_ld32(bool ok, uint32_t tm, float (&v)[32], int used) {
+  if (!ok) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fc00000);
+    return;
+  }
   tmem_ld32(tm, v);
   if constexpr (ACC > 1) {
     for (int a = 1; a < used; ++a) {
@@ -409,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (++st == STAGES) { st = 0; phase ^= 1; }
           }
         }
+        if (!ok) break;  // the tile is not complete
         if constexpr (PAIR) umma_commit_pair(acc_full(as));
         else umma_commit(acc_full(as));
       }
@@ -418,12 +429,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int part = w >> 2;                        // its half of the columns
     uint4* const stage = reinterpret_cast<uint4*>(generic + STAGES * STAGE + w * (kStaging / kEpiWarps));
     int seq = 0;
+    bool ok = true;
     for (int i = first_tile; i < t.total; i += tile_step, ++seq) {
-      const TileAt at = tile_at(t, i, seq);
+      TileAt at = tile_at(t, i, seq);
       const int as = BUFS == 2 ? seq & 1 : 0, row0 = at.m * (BM * CTAS) + (int)rank * BM + q * 32;
       typename Epi::Pre pre;
       Epi::prefetch(ep, t, at, row0, part, pre);
-      if (!mbar_wait(acc_full(as), (seq / BUFS) & 1, err, 15)) break;
+      at.ok = ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full(as), (seq / BUFS) & 1, err, 15));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       Epi::run(ep, t, at, tmem + as * 256 + ((uint32_t)(q * 32) << 16), row0, part, stage, pre);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -441,6 +453,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
+}
+
+// Reads and clears this file's error word in one step, so that no code is lost between the two.
+static __global__ void take_error_kernel(int* out) { *out = atomicExch(&error_word, 0); }
+
+// 0, or the code of a bounded wait that ran out since the last call.  Covers what was launched on the current stream of `like`'s
+// device, or on streams that it has waited for; waits for that work.
+inline int64_t take_error(const at::Tensor& like) {
+  c10::cuda::CUDAGuard guard(like.device());
+  at::Tensor word = at::empty({1}, like.options().dtype(at::kInt));
+  take_error_kernel<<<1, 1, 0, at::cuda::getCurrentCUDAStream()>>>(word.data_ptr<int>());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return word.item<int>();
 }
 
 // For epilogues that read nothing.
@@ -467,7 +492,7 @@ struct EpiStore : NoPrefetch {
     for (int cb = 0; cb < COLS / 32; ++cb) {
       const int c = part * COLS + cb * 32, n0 = at.n * BN + c;
       float v[32];
-      acc_ld32<ACC, BN>(tm + c, v, used);
+      acc_ld32<ACC, BN>(at.ok, tm + c, v, used);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= p.alpha;
       uint4 o[Slots<T>::n];

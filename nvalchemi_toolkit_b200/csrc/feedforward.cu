@@ -137,7 +137,8 @@ __device__ __forceinline__ void store_cols(uint4* stage, float (&v)[C], void* ds
   }
 }
 
-// Columns [0, BN/2) of the accumulator: g, [BN/2, BN): u, both of the same BN/2 columns of h.
+// Columns [0, BN/2) of the accumulator: g, [BN/2, BN): u, both of the same BN/2 columns of h.  (After an expired wait g alone is
+// replaced by NaN, here and below: every result depends on it.)
 template <typename T, int BN>
 struct EpiGated : NoPrefetch {
   static constexpr int kAcc = sizeof(T) == 4 ? 512 / BN : 1, kStride = BN;
@@ -150,8 +151,8 @@ struct EpiGated : NoPrefetch {
     for (int cb = 0; cb < BN / 128; ++cb) {
       const int c = part * (BN / 4) + cb * 32, n0 = at.n * (BN / 2) + c;
       float g[32], u[32];
-      acc_ld32<kAcc, kStride>(tm + c, g, used);
-      acc_ld32<kAcc, kStride>(tm + BN / 2 + c, u, used);
+      acc_ld32<kAcc, kStride>(at.ok, tm + c, g, used);
+      acc_ld32<kAcc, kStride>(true, tm + BN / 2 + c, u, used);
       if (p.act == kSilu) gate<sizeof(T) == 4, kSilu>(g, u);
       else gate<sizeof(T) == 4, kGelu>(g, u);
       store_cols<T>(stage, g, p.h, (int64_t)row0 * p.ld + n0, p.ld, p.plane, t.M - row0, t.N - n0, p.two);
@@ -185,7 +186,7 @@ struct EpiGatedGrad : NoPrefetch {
     for (int cb = 0; cb < 2; ++cb) {
       const int c = part * 64 + cb * 32;
       float g[32], u[32], d[32];
-      tmem_ld32(tm + c, g);
+      acc_ld32<1, 0>(at.ok, tm + c, g, 1);
       tmem_ld32(tm + 128 + c, u);
       tmem_ld32(td + c, d);
       store_grads<T>(p, t, row0, at.n * 128 + c, stage, g, u, d);
@@ -217,8 +218,8 @@ struct EpiGatedGradRead {
 #pragma unroll
       for (int j = 0; j < 32; ++j) d[j] = reinterpret_cast<const float*>(pre.raw)[j];
       if (cb + 1 < BN / 128) fetch(p, t, row0, n0 + 32, pre);
-      acc_ld32<kAcc, kStride>(tm + c, g, used);
-      acc_ld32<kAcc, kStride>(tm + BN / 2 + c, u, used);
+      acc_ld32<kAcc, kStride>(at.ok, tm + c, g, used);
+      acc_ld32<kAcc, kStride>(true, tm + BN / 2 + c, u, used);
       store_grads<float>(p.out, t, row0, n0, stage, g, u, d);
     }
   }
@@ -555,14 +556,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
   return {dx, dgu.select(0, 0), dgu.select(0, 1), dwd};
 }
 
-// Reads (and clears) the error word of this file's kernels: 0 = no bounded wait expired since the last call.
-int64_t gated_ff_error_status(const Tensor& like) {
-  c10::cuda::CUDAGuard guard(like.device());
-  int v = 0, zero = 0;
-  C10_CUDA_CHECK(cudaMemcpyFromSymbol(&v, dense::error_word, sizeof(int)));
-  if (v != 0) C10_CUDA_CHECK(cudaMemcpyToSymbol(dense::error_word, &zero, sizeof(int)));
-  return v;
-}
+int64_t gated_ff_error_status(const Tensor& like) { return dense::take_error(like); }
 
 }  // namespace nva
 

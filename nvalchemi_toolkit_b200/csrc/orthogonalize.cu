@@ -62,7 +62,7 @@ struct EpiGram : NoPrefetch {
     for (int cb = 0; cb < BN / 64; ++cb) {
       const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c;
       float v[32], dg = 0.f;
-      tmem_ld32(tm + c, v);
+      acc_ld32<1, 0>(at.ok, tm + c, v, 1);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         v[j] *= 1.f / kXScale;  // accumulated 2^24 A
@@ -105,7 +105,7 @@ struct EpiPoly {
       const float dl = pre.dl;
       if (cb + 1 < BN / 64) fetch(p, t, at, row0, n0 + 32, pre);
       float v[32], dg = 0.f;
-      tmem_ld32(tm + c, v);
+      acc_ld32<1, 0>(at.ok, tm + c, v, 1);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         const float aa = v[j] * (1.f / (kXScale * kXScale));
@@ -163,7 +163,7 @@ struct EpiUpdate {
       const float bl = pre.bl;
       if (cb + 1 < BN / 64) fetch(p, t, at, row0, n0 + 32, pre);
       float v[32];
-      tmem_ld32(tm + c, v);
+      acc_ld32<1, 0>(at.ok, tm + c, v, 1);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {  // 2^12 X
         const float h = __half2float(reinterpret_cast<const __half*>(h4)[j]), l = __half2float(reinterpret_cast<const __half*>(l4)[j]);
@@ -471,10 +471,12 @@ __global__ void __launch_bounds__(kSmallThreads)
     }
     publish();
   }
+  __nv_bfloat16* dst = out + blockIdx.x * (int64_t)count;
   if (__syncthreads_and(ok)) {
-    __nv_bfloat16* dst = out + blockIdx.x * (int64_t)count;
 #pragma unroll 4
     for (int i = threadIdx.x; i < count; i += kSmallThreads) dst[i] = *reinterpret_cast<const __nv_bfloat16*>(xh + place(i));
+  } else {  // a wait ran out: nothing finite that was not computed
+    for (int i = threadIdx.x; i < count; i += kSmallThreads) dst[i] = __ushort_as_bfloat16(0x7fc0);
   }
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
@@ -598,13 +600,7 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
   return out;
 }
 
-int64_t newton_schulz_error_status(const Tensor& like) {
-  c10::cuda::CUDAGuard guard(like.device());
-  int v = 0, zero = 0;
-  C10_CUDA_CHECK(cudaMemcpyFromSymbol(&v, dense::error_word, sizeof(int)));
-  if (v != 0) C10_CUDA_CHECK(cudaMemcpyToSymbol(dense::error_word, &zero, sizeof(int)));
-  return v;
-}
+int64_t newton_schulz_error_status(const Tensor& like) { return dense::take_error(like); }
 
 }  // namespace nva
 

@@ -166,7 +166,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
 
 
 def check_errors(like: torch.Tensor) -> int:
-    """Status word of the kernels on ``like``'s device (0 = fine; non-zero = a bounded wait expired)."""
+    """Status word of the kernels on ``like``'s device (0 = fine; non-zero = a bounded wait expired and NaN stands where nothing was
+    formed).  Covers work launched on the current stream, or on streams it has waited for; waits for it and clears the word."""
     if like.is_cuda and _native.available():
         return int(_nops.gated_ff_error_status(like))
     return 0

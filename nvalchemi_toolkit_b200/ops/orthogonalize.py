@@ -80,7 +80,8 @@ def _formula(x: torch.Tensor, steps: int, a: float, b: float, c: float, eps: flo
 
 
 def check_errors(like: torch.Tensor) -> int:
-    """Status word of the kernels on ``like``'s device (0 = fine; non-zero = a bounded wait expired)."""
+    """Status word of the kernels on ``like``'s device (0 = fine; non-zero = a bounded wait expired and NaN stands where nothing was
+    formed).  Covers work launched on the current stream, or on streams it has waited for; waits for it and clears the word."""
     if like.is_cuda and _native.available():
         return int(_nops.newton_schulz_error_status(like))
     return 0

@@ -17,6 +17,7 @@ import torch
 
 from nvalchemi_toolkit_b200._serialization import import_from_path, type_to_path
 from nvalchemi_toolkit_b200.hooks.core import HookRegistryMixin, TrainContext
+from nvalchemi_toolkit_b200.ops import status
 from nvalchemi_toolkit_b200.training import checkpoint as ckpt
 from nvalchemi_toolkit_b200.training._stages import TrainingStage
 from nvalchemi_toolkit_b200.training.distributed import get_rank, get_world_size
@@ -231,8 +232,13 @@ class TrainingStrategy(HookRegistryMixin):
                 self._maybe_validate(TrainingStage.AFTER_EPOCH, validation_dataloader)
             if per_epoch == 0:
                 break
+        self._check_kernels()
         self._run_hooks(TrainingStage.AFTER_TRAINING, None)
         return self
+
+    def _check_kernels(self) -> None:
+        """Raise when a kernel's bounded wait has run out since the last look (``ops/status.py``)."""
+        status.raise_on_kernel_errors(torch.empty(0, device=self.devices[0]))
 
     # ---- validation ---------------------------------------------------------------------------------------
     def _maybe_validate(self, stage: TrainingStage, loader: Iterable | None) -> None:
@@ -257,6 +263,7 @@ class TrainingStrategy(HookRegistryMixin):
             return None
         with ValidationLoop.from_training_strategy(self, cfg) as loop:
             summary = loop.run(loader)
+        self._check_kernels()
         self.last_validation = summary
         step_schedulers(self._lr_schedulers, self._opt_cfgs, "validation", summary)
         self._run_hooks(TrainingStage.AFTER_VALIDATION, None)
@@ -291,7 +298,10 @@ class TrainingStrategy(HookRegistryMixin):
 
     def save_checkpoint(self, directory: str | Path, asynchronous: bool = False) -> "Path | ckpt.PendingCheckpoint":
         """Rank 0 writes the checkpoint; ``asynchronous=True`` snapshots to host memory and returns a handle whose
-        ``wait()`` joins the background writer."""
+        ``wait()`` joins the background writer.  Raises instead of writing when a kernel has reported an expired wait (not
+        asked for an asynchronous checkpoint, which must not wait for the GPU)."""
+        if not asynchronous:
+            self._check_kernels()
         if get_rank(self.distributed_manager) != 0:
             return Path(directory)
         return ckpt.save_checkpoint(directory, self.step_count, self.models, self._optimizers, self._lr_schedulers,

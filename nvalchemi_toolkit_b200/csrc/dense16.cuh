@@ -8,11 +8,11 @@
 // values is 64 rows of 128 swizzled bytes in both cases, only the coordinates and the matrix descriptors differ, so no
 // operand is transposed in memory.
 //
-// The tensor core cuts an accumulator to 24 bits after every instruction, towards zero: after n instructions a sum has lost
-// about n / 3 of half a step, always in the same direction.  That is nothing beside a 16-bit result, and 1.1e-5 of a float32
-// one of 6 x 1024 terms (measured).  So a float32 product adds its five small partial products first, while the sum is small,
-// and deals the large one out over up to four accumulators that the epilogue adds in fp32; longer contraction axes are split
-// over several tiles.
+// The tensor core cuts what it adds to an accumulator towards zero: where all terms have one sign, an instruction loses up to
+// 1.7 half steps of the sum so far (2^-24 of it; measured: 1.7e-3 of a sum of 16,384 instructions, 6.5e-3 of 65,536, always in the
+// same direction).  So a float32 product adds its five small partial products first, while the sum is small, and deals the large
+// one out over up to four accumulators that the epilogue adds in fp32.  max_blocks() below says how much one accumulator may
+// take; a longer contraction axis is split over several tiles, whose partial sums are added in fp32.
 //
 // One persistent CTA per SM: warp 0 loads tiles by TMA into a ring of stages, one lane of warp 1 issues tcgen05.mma
 // (K = 16 per instruction), warps 2..9 are the epilogue (16 warps
@@ -65,6 +65,7 @@ struct Tiles {
   int mt, nt, bn;        // tiles along each, columns of a tile
   int bm;                // rows of a tile: 128, or 256 for a pair of CTAs
   int batches, splits, total;
+  int split0;            // the first of the launch's splits
   int lower;             // symmetric output, only tiles that reach the diagonal or lie below it: bm / bn, else 0
   int n_seg;
   int main_nk[2];        // nk of the spread segments of each group
@@ -99,7 +100,7 @@ __device__ __forceinline__ TileAt tile_at(const Tiles& t, int i, int seq) {
   const int z = i / per;
   const int j = i - z * per;
   r.batch = z % t.batches;
-  r.split = z / t.batches;
+  r.split = t.split0 + z / t.batches;
   if (t.lower) {  // row m holds lower * (m + 1) tiles
     const int k = j / t.lower;
     int m = (int)((sqrtf(8.f * (float)k + 1.f) - 1.f) * 0.5f);
@@ -485,7 +486,7 @@ struct EpiStore : NoPrefetch {
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
     constexpr int COLS = BN / 2;  // columns of a warp
-    T* out = p.out + at.batch * p.batch_stride + at.split * p.split_stride;
+    T* out = p.out + at.batch * p.batch_stride + (at.split - t.split0) * p.split_stride;
     const bool vec_ok = p.ld % (16 / (int)sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     const int used = used_acc<ACC>(t, at, 0);
 #pragma unroll 1
@@ -555,7 +556,7 @@ inline void set_tiles(Tiles& t, int64_t M, int64_t N, int bn, int64_t batches, i
   t.M = (int)M; t.N = (int)N; t.bn = bn;
   t.bm = pair && use_pair(M) ? 2 * BM : BM;
   t.mt = (int)((M + t.bm - 1) / t.bm); t.nt = (int)((N + bn - 1) / bn);
-  t.batches = (int)batches; t.splits = splits; t.lower = lower ? t.bm / bn : 0;
+  t.batches = (int)batches; t.splits = splits; t.split0 = 0; t.lower = lower ? t.bm / bn : 0;
   TORCH_CHECK(!lower || (t.lower >= 1 && t.bm % bn == 0), "dense: symmetric tiles do not fit");
   const int64_t per = lower ? (int64_t)t.lower * ((int64_t)t.mt * (t.mt + 1) / 2) : (int64_t)t.mt * t.nt;
   TORCH_CHECK(per * batches * splits < (1ll << 31), "dense: too many tiles");
@@ -593,6 +594,11 @@ inline int pick_bn(int64_t tiles256, int64_t tiles128) {
   const double wide = (double)((tiles256 + pairs - 1) / pairs), narrow = 0.7 * (double)((tiles128 + pairs - 1) / pairs);
   return wide <= narrow ? 256 : 128;
 }
+
+// 64-wide blocks (four instructions each) that may be added to one accumulator.  16 bits: what is lost stays under an eighth of
+// half a step of the result's type, 2^-14 (float16) and 2^-11.  float32: 32 instructions, 7e-7 in sums of both signs and 3.2e-6
+// at most.
+inline int max_blocks(at::ScalarType t) { return t == at::kFloat ? 8 : t == at::kHalf ? 128 : 1024; }
 
 // Tiles that run at the same time.
 inline int slots(const Tiles& t) { return t.bm == BM ? sm_count() : sm_count() / 2; }

@@ -12,6 +12,9 @@
 // own rounding); up to 256 rows, where the products cost next to nothing, they are kept as a 16-bit value and a 16-bit
 // remainder and the next product reads both.
 //
+// Where the contraction axis of a projection (K, or N for dh) is too long for the accumulators of one tile (max_blocks), g, u and
+// dh are formed as float32 matrices by split products and a kernel of its own applies the gate.
+//
 // float32 matrices run on the same tensor cores: a value is the exact sum of three bf16 values and a product the six
 // partial products down to 2^-24; the intermediate h, dg and du are stored as three planes each, so nothing is lost to
 // 16 bits.  There dh is a product of its own (its accumulators would not fit beside those of g and u).
@@ -262,13 +265,13 @@ void run_packs(const PackJobs& jobs, int planes, cudaStream_t st) {
   launch_chained(planes == 3 ? pack_kernel<float, 3> : pack_kernel<__half, 1>, grid, 256, st, jobs);
 }
 
-// out = sum over splits of partial [splits][n], in order.
+// out = base (0 if null) + the sum over splits of partial [splits][n], in order.  `base` may be `out`.
 template <typename T>
-__global__ void split_sum_kernel(const float* __restrict__ partial, int splits, int64_t stride, int64_t n, T* __restrict__ out) {
+__global__ void split_sum_kernel(const float* __restrict__ partial, int splits, int64_t stride, int64_t n, const float* base, T* out) {
   chain_wait();
   const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
   if (i >= n) return;
-  float s = 0.f;
+  float s = base != nullptr ? base[i] : 0.f;
   for (int k = 0; k < splits; ++k) s += partial[k * stride + i];
   out[i] = narrow<T>(s);
 }
@@ -362,28 +365,41 @@ struct Plan {
 };
 
 // Plain product into `out` [batches][M][N].  The contraction axis is split over several tiles (partials added in order by a
-// second kernel) when half of the GPU or more would have no tile and the axis is long, and for float32 so that no accumulator
-// takes more than 32 instructions of the large partial product (up to 64 partials: 131,072 terms in sums of 64 instructions).
+// second kernel) when half of the GPU or more would have no tile and the axis is long, and so that no accumulator takes more
+// than max_blocks.  More than kPartials partials are formed and added in several rounds.
+constexpr int kPartials = 64;
 template <typename T, int BN, int ACC>
 void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   set_tiles(pl.t, M, N, BN, batches, 1);
   const int tiles = pl.t.total, nk = pl.t.main_nk[0], kb = nk * pl.t.n_seg, at_once = slots(pl.t);
   int mains = 0;  // large partial products that add to the same accumulators
   for (int i = 0; i < pl.t.n_seg; ++i) mains += pl.t.seg[i].spread;
+  const int limit = max_blocks(out.scalar_type()) * ACC, load = nk * (ACC > 1 ? mains : pl.t.n_seg);
   int splits = 1;
-  if (2 * tiles <= at_once) splits = std::max(1, std::min({at_once / tiles, kb / 8, nk, 64}));
-  if (ACC > 1) splits = std::min({nk, 64, std::max(splits, (nk * mains + 8 * ACC - 1) / (8 * ACC))});
+  if (2 * tiles <= at_once) splits = std::max(1, std::min({at_once / tiles, kb / 8, nk, kPartials}));
+  splits = std::min(nk, std::max(splits, (load + limit - 1) / limit));
   if (splits == 1) {
     typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
     run_dense<BN, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);
     return;
   }
-  set_tiles(pl.t, M, N, BN, batches, splits);
   const int64_t n = batches * M * N;
-  Tensor part = at::empty({splits, n}, out.options().dtype(at::kFloat));
-  typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n, 1.f};
-  run_dense<BN, EpiStore<float, BN, ACC>>(pl.maps, pl.t, ep, st);
-  launch_chained(split_sum_kernel<T>, dim3((unsigned)((n + 255) / 256)), 256, st, part.data_ptr<float>(), splits, n, n, (T*)out.data_ptr());
+  Tensor part = at::empty({std::min(splits, kPartials), n}, out.options().dtype(at::kFloat)), total;
+  if (splits > kPartials) total = sizeof(T) == 4 ? out : at::empty({n}, part.options());
+  const dim3 grid((unsigned)((n + 255) / 256));
+  for (int s0 = 0; s0 < splits; s0 += kPartials) {
+    const int here = std::min(kPartials, splits - s0);
+    set_tiles(pl.t, M, N, BN, batches, here);
+    pl.t.splits = splits;
+    pl.t.split0 = s0;
+    typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n, 1.f};
+    run_dense<BN, EpiStore<float, BN, ACC>>(pl.maps, pl.t, ep, st);
+    const float* const base = s0 > 0 ? total.data_ptr<float>() : nullptr;
+    if (s0 + here < splits)
+      launch_chained(split_sum_kernel<float>, grid, 256, st, part.data_ptr<float>(), here, n, n, base, total.data_ptr<float>());
+    else
+      launch_chained(split_sum_kernel<T>, grid, 256, st, part.data_ptr<float>(), here, n, n, base, (T*)out.data_ptr());
+  }
 }
 
 // Columns of a tile of an M x N product over `kb` blocks of the contraction axis (all segments): by the number of tiles, and 256
@@ -407,6 +423,73 @@ void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_
   };
   if (out.scalar_type() == at::kFloat) go(float{});
   else if (out.scalar_type() == at::kHalf) go(__half{});
+  else go(__nv_bfloat16{});
+}
+
+// Whether a projection over an axis of K is too long for the accumulators of one tile (float32: two of them).
+bool far(const Tensor& x, int64_t K) { return (K + BK - 1) / BK > max_blocks(x.scalar_type()) * (x.scalar_type() == at::kFloat ? 2 : 1); }
+
+// out [M][N] float32 = a . b over axes 1 and `kb`.
+void project(bool bf16, const Operand& a, const Operand& b, int kb, Tensor& out, cudaStream_t st) {
+  Plan pl(bf16);
+  const int64_t M = out.size(0), N = out.size(1);
+  const int bn = store_bn(1, M, N, blocks_of(a.planes, a.extent(1)));
+  const int ia = pl.map(a), ib = pl.map(b);
+  pl.product(ia, a, 1, ib, -1, b, kb, 0, bn);
+  store_any(pl, bn, out, 1, M, N, st);
+}
+
+// The gate on float32 matrices g, u [M][H] (and dh [M][ld_dh]): h, or dg, du and h.
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ gm, const float* __restrict__ um, const float* __restrict__ dm,
+                                                   int64_t ld_dh, int64_t M, int64_t H, const __grid_constant__ GradOut out) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  chain_wait();
+  auto put = [&](void* dst, int64_t at, float v) {
+    if constexpr (EXACT) {
+      float p[3];
+      split3(v, p[0], p[1], p[2]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) ((__nv_bfloat16*)dst)[at + k * out.plane] = __float2bfloat16_rn(p[k]);
+    } else {
+      ((T*)dst)[at] = narrow<T>(v);
+      if (out.two) ((T*)dst)[at + out.plane] = narrow<T>(v - widen(narrow<T>(v)));
+    }
+  };
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < M * H; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / H, c = i - r * H, at = r * out.ld + c;
+    float g[1] = {gm[i]}, u[1] = {um[i]};
+    if constexpr (GRAD) {
+      float d[1] = {dm[r * ld_dh + c]};
+      if (out.act == kSilu) gate_grad<EXACT, kSilu>(g, u, d);
+      else gate_grad<EXACT, kGelu>(g, u, d);
+      put(out.dg, at, g[0]);
+      put(out.du, at, d[0]);
+      put(out.h, at, u[0]);
+    } else {
+      if (out.act == kSilu) gate<EXACT, kSilu>(g, u);
+      else gate<EXACT, kGelu>(g, u);
+      put(out.h, at, g[0]);
+    }
+  }
+}
+// g = x Wg and u = x Wu through memory, then the gate (dh: float32 [M][ld_dh], or undefined for the forward pass).
+void gate_through_memory(const Tensor& x, const Operand& ox, const Operand& og, const Operand& ou, const Tensor& dh, int64_t H,
+                         const GradOut& out, cudaStream_t st) {
+  const int64_t M = x.size(0);
+  Tensor gu = at::empty({2, M, H}, x.options().dtype(at::kFloat)), g = gu.select(0, 0), u = gu.select(0, 1);
+  project(x.scalar_type() != at::kHalf, ox, og, 0, g, st);
+  project(x.scalar_type() != at::kHalf, ox, ou, 0, u, st);
+  const dim3 grid((unsigned)std::min<int64_t>((M * H + 255) / 256, 148 * 8));
+  auto go = [&](auto v) {
+    using T = decltype(v);
+    if (dh.defined())
+      launch_chained(gate_kernel<T, true>, grid, 256, st, g.data_ptr<float>(), u.data_ptr<float>(), dh.data_ptr<float>(), dh.size(1), M, H, out);
+    else
+      launch_chained(gate_kernel<T, false>, grid, 256, st, g.data_ptr<float>(), u.data_ptr<float>(), (const float*)nullptr, (int64_t)0, M, H, out);
+  };
+  if (x.scalar_type() == at::kFloat) go(float{});
+  else if (x.scalar_type() == at::kHalf) go(__half{});
   else go(__nv_bfloat16{});
 }
 
@@ -435,7 +518,7 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
   check_ff(x_in, wg, wu, wd, act);
   c10::cuda::CUDAGuard guard(x_in.device());
   const Tensor x = as_matrix(x_in);
-  const int64_t M = x.size(0), H = wg.size(1), N = wd.size(1);
+  const int64_t M = x.size(0), K = x.size(1), H = wg.size(1), N = wd.size(1);
   Tensor y = at::empty(out_sizes(x_in, N), x.options());
   if (M == 0) return y;
   auto st = at::cuda::getCurrentCUDAStream();
@@ -447,7 +530,9 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
   run_packs(jobs, P, st);
   const int Pi = parts_of(P, M);
   Operand oh = intermediate(M, H, Pi, x);
-  {
+  if (far(x, K)) {
+    gate_through_memory(x, ox, og, ou, Tensor(), H, {nullptr, nullptr, oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act, Pi == 2 ? 1 : 0}, st);
+  } else {
     Plan pl(bf16);
     const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou);
     auto go = [&](auto v, auto bn_tag) {
@@ -500,7 +585,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
   Operand oe = intermediate(M, H, Pi, x, 2), oh = intermediate(M, H, Pi, x);  // dg then du; h
   uint16_t* const e = (uint16_t*)oe.keep.data_ptr();
   const GradOut out{e, e + Pi * oe.s.plane, oh.keep.data_ptr(), oh.s.ld, oh.s.plane, (int)act, Pi == 2 ? 1 : 0};
-  if (P == 1) {
+  const bool through_memory = far(x, K) || (P == 1 && far(x, N));
+  if (P == 1 && !through_memory) {
     Plan pl(bf16);
     const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou), a3 = pl.map(oy), b3 = pl.map(od);
     pl.product(a3, oy, 1, b3, -1, od, 1, 256, 128, 0, 0, 0, 0, 2, 1);
@@ -510,24 +596,22 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
     else run_dense<256, EpiGatedGrad<__half>>(pl.maps, pl.t, out, st);
   } else {
     const int64_t ld_dh = (H + 3) / 4 * 4;  // columns past H come out as zeros
-    Tensor dh = at::empty({M, ld_dh}, x.options());
-    {
+    Tensor dh = at::empty({M, ld_dh}, x.options().dtype(at::kFloat));
+    project(bf16, oy, od, 1, dh, st);
+    if (through_memory) {
+      gate_through_memory(x, ox, og, ou, dh, H, out, st);
+    } else {
       Plan pl(bf16);
-      const int bn = store_bn(1, M, ld_dh, blocks_of(P, N));
-      const int a = pl.map(oy), b = pl.map(od);
-      pl.product(a, oy, 1, b, -1, od, 1, 0, bn);
-      store_any(pl, bn, dh, 1, M, ld_dh, st);
+      const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou);
+      auto go = [&](auto bn_tag) {
+        constexpr int BN = decltype(bn_tag)::value;
+        pl.product(a, ox, 1, b, b2, og, 0, 0, BN);
+        set_tiles(pl.t, M, H, BN / 2, 1, 1);
+        run_dense<BN, EpiGatedGradRead<BN>>(pl.maps, pl.t, {out, dh.data_ptr<float>(), ld_dh}, st);
+      };
+      if (store_bn(1, M, 2 * H, 0) == 256) go(std::integral_constant<int, 256>{});
+      else go(std::integral_constant<int, 128>{});
     }
-    Plan pl(bf16);
-    const int a = pl.map(ox), b = pl.map(og), b2 = pl.map(ou);
-    auto go = [&](auto bn_tag) {
-      constexpr int BN = decltype(bn_tag)::value;
-      pl.product(a, ox, 1, b, b2, og, 0, 0, BN);
-      set_tiles(pl.t, M, H, BN / 2, 1, 1);
-      run_dense<BN, EpiGatedGradRead<BN>>(pl.maps, pl.t, {out, dh.data_ptr<float>(), ld_dh}, st);
-    };
-    if (store_bn(1, M, 2 * H, 0) == 256) go(std::integral_constant<int, 256>{});
-    else go(std::integral_constant<int, 128>{});
   }
   if (which & 1) {
     Plan pl(bf16);

@@ -27,8 +27,7 @@
 // 32 KB per CTA.
 //
 // Every wait is bounded; on expiry the error word is set, the products stop, the producer waits (bounded) for its copies in
-// flight, the epilogue goes on with NaN in the place of the accumulators (no finite result is left that nothing has formed), and
-// the TMEM is freed.
+// flight, the epilogue stores NaN for this tile and the CTA's remaining ones, and the TMEM is freed.
 #pragma once
 #include "common.cuh"
 #include "convert.cuh"
@@ -74,10 +73,7 @@ struct Tiles {
 
 struct alignas(64) Maps { CUtensorMap m[kMaxMaps]; int n = 0; };
 
-struct TileAt {
-  int m, n, batch, split, seq;  // seq: the CTA's how-manieth tile
-  bool ok;                      // its products are done; false after an expired wait, the same for all lanes of a warp
-};
+struct TileAt { int m, n, batch, split, seq; };  // seq: the CTA's how-manieth tile
 
 // The part of a segment's blocks that one of `splits` tiles of the same output takes.
 __device__ __forceinline__ int split_at(int nk, int split, int splits) {
@@ -95,7 +91,6 @@ __device__ __forceinline__ int used_acc(const Tiles& t, const TileAt& at, int gr
 __device__ __forceinline__ TileAt tile_at(const Tiles& t, int i, int seq) {
   TileAt r;
   r.seq = seq;
-  r.ok = true;
   const int per = t.lower ? t.lower * (t.mt * (t.mt + 1) / 2) : t.mt * t.nt;
   const int z = i / per;
   const int j = i - z * per;
@@ -267,14 +262,9 @@ __device__ __forceinline__ void split3(float v, float& p0, float& p1, float& p2)
   p2 = r - p1;
 }
 
-// 32 columns of the sum of a group's accumulators, STRIDE columns apart; NaN after an expired wait.
+// 32 columns of the sum of a group's accumulators, STRIDE columns apart.
 template <int ACC, int STRIDE>
-__device__ __forceinline__ void acc_ld32(bool ok, uint32_t tm, float (&v)[32], int used) {
-  if (!ok) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fc00000);
-    return;
-  }
+__device__ __forceinline__ void acc_ld32(uint32_t tm, float (&v)[32], int used) {
   tmem_ld32(tm, v);
   if constexpr (ACC > 1) {
     for (int a = 1; a < used; ++a) {
@@ -286,9 +276,28 @@ __device__ __forceinline__ void acc_ld32(bool ok, uint32_t tm, float (&v)[32], i
   }
 }
 
+// NaN in `cols` columns of a warp's 32 rows.
+template <typename T>
+__device__ __forceinline__ void fill_nan(T* dst, int64_t ld, int rows_left, int cols_left, int cols) {
+  const int row = threadIdx.x & 31;
+  if (row >= rows_left) return;
+#pragma unroll 1
+  for (int c = 0; c < min(cols, cols_left); ++c) dst[row * ld + c] = narrow<T>(__int_as_float(0x7fc00000));
+}
+
+// NaN in an epilogue warp's part of the tiles from `i` on: a function of its own, so that the kernel keeps its registers.
+template <int CTAS, typename Epi>
+__device__ __noinline__ void poison_tiles(const Tiles& t, const typename Epi::Params& ep, int i, int step, int rank, int w) {
+  for (; i < t.total; i += step) {
+    const TileAt at = tile_at(t, i, 0);
+    Epi::poison(ep, t, at, at.m * (BM * CTAS) + rank * BM + ((w + 2) & 3) * 32, w >> 2);
+  }
+}
+
 // Epi::kAcc accumulators per column group, kStride columns apart; Epi::kLate: see below; Epi::Params; Epi::Pre: what
 // Epi::prefetch(params, tiles, tile, first row of the warp, share of the columns, pre) reads before the tile's products are done;
-// Epi::run(params, tiles, tile, tmem (lane quarter added), first row, share, stage, pre).
+// Epi::run(params, tiles, tile, tmem (lane quarter added), first row, share, stage, pre); Epi::poison(params, tiles, tile, first
+// row, share): NaN in what `run` would store.
 //
 // kLate: a tile fills TMEM columns 0..383, group 0 in 0..255 and group 1 (whose segments come first) in the 128 columns after
 // those, in turns with the last 128, so that the next tile's group 1 is formed while the epilogue still reads this tile.
@@ -310,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0;
   const int first_tile = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
+  int unformed = t.total;  // an epilogue warp's first tile that was not formed
   int* const err = &error_word;
 
   // The next kernel of the chain may start on idle SMs and set itself up; it waits below until this one is done.
@@ -429,14 +439,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = warp - 2, q = warp & 3;  // q: the TMEM lanes this warp may read
     const int part = w >> 2;                        // its half of the columns
     uint4* const stage = reinterpret_cast<uint4*>(generic + STAGES * STAGE + w * (kStaging / kEpiWarps));
-    int seq = 0;
-    bool ok = true;
-    for (int i = first_tile; i < t.total; i += tile_step, ++seq) {
-      TileAt at = tile_at(t, i, seq);
+    int seq = 0, i = first_tile;
+    for (; i < t.total; i += tile_step, ++seq) {
+      const TileAt at = tile_at(t, i, seq);
       const int as = BUFS == 2 ? seq & 1 : 0, row0 = at.m * (BM * CTAS) + (int)rank * BM + q * 32;
       typename Epi::Pre pre;
       Epi::prefetch(ep, t, at, row0, part, pre);
-      at.ok = ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_full(as), (seq / BUFS) & 1, err, 15));
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full(as), (seq / BUFS) & 1, err, 15))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       Epi::run(ep, t, at, tmem + as * 256 + ((uint32_t)(q * 32) << 16), row0, part, stage, pre);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -446,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         else mbar_arrive(acc_empty(as));
       }
     }
+    unformed = i;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -454,6 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
+  if (unformed < t.total) poison_tiles<CTAS, Epi>(t, ep, unformed, tile_step, (int)rank, warp - 2);
 }
 
 // Reads and clears this file's error word in one step, so that no code is lost between the two.
@@ -483,6 +494,11 @@ struct EpiStore : NoPrefetch {
   static constexpr bool kLate = false;
   static_assert(ACC == 1 || ACC * BN <= 512, "dense: accumulators exceed the TMEM");
   struct Params { T* out; int64_t ld, batch_stride, split_stride; float alpha; };
+  static __device__ __forceinline__ void poison(const Params& p, const Tiles& t, const TileAt& at, int row0, int part) {
+    const int n0 = at.n * BN + part * (BN / 2);
+    fill_nan(p.out + at.batch * p.batch_stride + (at.split - t.split0) * p.split_stride + (int64_t)row0 * p.ld + n0, p.ld, t.M - row0,
+             t.N - n0, BN / 2);
+  }
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
     constexpr int COLS = BN / 2;  // columns of a warp
@@ -493,7 +509,7 @@ struct EpiStore : NoPrefetch {
     for (int cb = 0; cb < COLS / 32; ++cb) {
       const int c = part * COLS + cb * 32, n0 = at.n * BN + c;
       float v[32];
-      acc_ld32<ACC, BN>(at.ok, tm + c, v, used);
+      acc_ld32<ACC, BN>(tm + c, v, used);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= p.alpha;
       uint4 o[Slots<T>::n];

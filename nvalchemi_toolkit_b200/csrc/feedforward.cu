@@ -140,13 +140,22 @@ __device__ __forceinline__ void store_cols(uint4* stage, float (&v)[C], void* ds
   }
 }
 
-// Columns [0, BN/2) of the accumulator: g, [BN/2, BN): u, both of the same BN/2 columns of h.  (After an expired wait g alone is
-// replaced by NaN, here and below: every result depends on it.)
+// NaN in `cols` columns of a warp's rows of an intermediate; its other planes need none, what reads them reads this one too.
+template <typename T>
+__device__ __forceinline__ void poison_cols(void* dst, int64_t ld, const Tiles& t, int row0, int n0, int cols) {
+  using S = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
+  fill_nan((S*)dst + (int64_t)row0 * ld + n0, ld, t.M - row0, t.N - n0, cols);
+}
+
+// Columns [0, BN/2) of the accumulator: g, [BN/2, BN): u, both of the same BN/2 columns of h.
 template <typename T, int BN>
 struct EpiGated : NoPrefetch {
   static constexpr int kAcc = sizeof(T) == 4 ? 512 / BN : 1, kStride = BN;
   static constexpr bool kLate = false;
   struct Params { void* h; int64_t ld, plane; int act, two; };
+  static __device__ __forceinline__ void poison(const Params& p, const Tiles& t, const TileAt& at, int row0, int part) {
+    poison_cols<T>(p.h, p.ld, t, row0, at.n * (BN / 2) + part * (BN / 4), BN / 4);
+  }
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
     const int used = used_acc<kAcc>(t, at, 0);
@@ -154,8 +163,8 @@ struct EpiGated : NoPrefetch {
     for (int cb = 0; cb < BN / 128; ++cb) {
       const int c = part * (BN / 4) + cb * 32, n0 = at.n * (BN / 2) + c;
       float g[32], u[32];
-      acc_ld32<kAcc, kStride>(at.ok, tm + c, g, used);
-      acc_ld32<kAcc, kStride>(true, tm + BN / 2 + c, u, used);
+      acc_ld32<kAcc, kStride>(tm + c, g, used);
+      acc_ld32<kAcc, kStride>(tm + BN / 2 + c, u, used);
       if (p.act == kSilu) gate<sizeof(T) == 4, kSilu>(g, u);
       else gate<sizeof(T) == 4, kGelu>(g, u);
       store_cols<T>(stage, g, p.h, (int64_t)row0 * p.ld + n0, p.ld, p.plane, t.M - row0, t.N - n0, p.two);
@@ -175,6 +184,11 @@ __device__ __forceinline__ void store_grads(const GradOut& p, const Tiles& t, in
   store_cols<T>(stage, u, p.h, off, p.ld, p.plane, t.M - row0, t.N - n0, p.two);
 }
 
+template <typename T>
+__device__ __forceinline__ void poison_grads(const GradOut& p, const Tiles& t, int row0, int n0, int cols) {
+  for (void* dst : {p.dg, p.du, p.h}) poison_cols<T>(dst, p.ld, t, row0, n0, cols);
+}
+
 // 16 bits: of 128 columns of h, g in accumulator columns [0, 128), u in [128, 256), dh after those, in turns in two places (see
 // dense_kernel).
 template <typename T>
@@ -182,6 +196,9 @@ struct EpiGatedGrad : NoPrefetch {
   static constexpr int kAcc = 1, kStride = 0;
   static constexpr bool kLate = true;
   using Params = GradOut;
+  static __device__ __forceinline__ void poison(const Params& p, const Tiles& t, const TileAt& at, int row0, int part) {
+    poison_grads<T>(p, t, row0, at.n * 128 + part * 64, 64);
+  }
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int part,
                                              uint4* stage, Pre&) {
     const uint32_t td = tm + 256 + (at.seq & 1) * 128;
@@ -189,7 +206,7 @@ struct EpiGatedGrad : NoPrefetch {
     for (int cb = 0; cb < 2; ++cb) {
       const int c = part * 64 + cb * 32;
       float g[32], u[32], d[32];
-      acc_ld32<1, 0>(at.ok, tm + c, g, 1);
+      tmem_ld32(tm + c, g);
       tmem_ld32(tm + 128 + c, u);
       tmem_ld32(td + c, d);
       store_grads<T>(p, t, row0, at.n * 128 + c, stage, g, u, d);
@@ -204,6 +221,9 @@ struct EpiGatedGradRead {
   static constexpr bool kLate = false;
   struct Params { GradOut out; const float* dh; int64_t ld_dh; };
   struct Pre { uint4 raw[8]; };  // 32 columns of dh
+  static __device__ __forceinline__ void poison(const Params& p, const Tiles& t, const TileAt& at, int row0, int part) {
+    poison_grads<float>(p.out, t, row0, at.n * (BN / 2) + part * (BN / 4), BN / 4);
+  }
   static __device__ __forceinline__ void fetch(const Params& p, const Tiles& t, int row0, int n0, Pre& pre) {
     fetch_piece<float, 8>(pre.raw, p.dh + (int64_t)row0 * p.ld_dh + n0, p.ld_dh, t.M - row0, t.N - n0);
   }
@@ -221,8 +241,8 @@ struct EpiGatedGradRead {
 #pragma unroll
       for (int j = 0; j < 32; ++j) d[j] = reinterpret_cast<const float*>(pre.raw)[j];
       if (cb + 1 < BN / 128) fetch(p, t, row0, n0 + 32, pre);
-      acc_ld32<kAcc, kStride>(at.ok, tm + c, g, used);
-      acc_ld32<kAcc, kStride>(true, tm + BN / 2 + c, u, used);
+      acc_ld32<kAcc, kStride>(tm + c, g, used);
+      acc_ld32<kAcc, kStride>(tm + BN / 2 + c, u, used);
       store_grads<float>(p.out, t, row0, n0, stage, g, u, d);
     }
   }

@@ -48,12 +48,24 @@ __device__ __forceinline__ void store_symmetric(uint4* stage, const float (&v)[3
   }
 }
 
+// NaN in a warp's part of a symmetric tile, its mirror image and its rows of the diagonal.
+__device__ __forceinline__ void poison_symmetric(__half* out, float* diag, int64_t ld, int size, int row0, int n0, int cols, bool mirror) {
+  fill_nan(out + (int64_t)row0 * ld + n0, ld, size - row0, size - n0, cols);
+  if (mirror)
+    for (int c = 0; c < cols; c += 32) fill_nan(out + (int64_t)(n0 + c) * ld + row0, ld, size - n0 - c, size - row0, 32);
+  fill_nan(diag + row0, 1, size - row0, 1, 1);
+}
+
 // R = A without its diagonal (times 2^12), diag(A).
 template <int BN>
 struct EpiGram : NoPrefetch {
   static constexpr int kAcc = 1, kStride = BN;
   static constexpr bool kLate = false;
   struct Params { __half* r; float* diag; int64_t ld, stride; };
+  static __device__ __forceinline__ void poison(const Params& p, const Tiles& t, const TileAt& at, int row0, int half) {
+    poison_symmetric(p.r + at.batch * p.stride, p.diag + at.batch * (int64_t)t.M, p.ld, t.M, row0, at.n * BN + half * (BN / 2), BN / 2,
+                     at.n < t.lower * at.m);
+  }
   static __device__ __forceinline__ void run(const Params& p, const Tiles& t, const TileAt& at, uint32_t tm, int row0, int half,
                                              uint4* stage, Pre&) {
     __half* out = p.r + at.batch * p.stride;
@@ -62,7 +74,7 @@ struct EpiGram : NoPrefetch {
     for (int cb = 0; cb < BN / 64; ++cb) {
       const int c = half * (BN / 2) + cb * 32, n0 = at.n * BN + c;
       float v[32], dg = 0.f;
-      acc_ld32<1, 0>(at.ok, tm + c, v, 1);
+      tmem_ld32(tm + c, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         v[j] *= 1.f / kXScale;  // accumulated 2^24 A
@@ -83,6 +95,10 @@ struct EpiPoly {
   static constexpr bool kLate = false;
   struct Params { const __half* r; const float* diag; __half* bo; float* bdiag; int64_t ld, stride; float b, c; };
   struct Pre { uint4 raw[4]; float dl; };  // 32 columns of R (rows are padded to 8), and of the diagonal
+  static __device__ __forceinline__ void poison(const Params& p, const Tiles& t, const TileAt& at, int row0, int half) {
+    poison_symmetric(p.bo + at.batch * p.stride, p.bdiag + at.batch * (int64_t)t.M, p.ld, t.M, row0, at.n * BN + half * (BN / 2), BN / 2,
+                     at.n < t.lower * at.m);
+  }
   static __device__ __forceinline__ void fetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int n0, Pre& pre) {
     const int lane = threadIdx.x & 31;
     fetch_piece<__half, 4>(pre.raw, p.r + at.batch * p.stride + (int64_t)row0 * p.ld + n0, p.ld, t.M - row0, t.M - n0);
@@ -105,7 +121,7 @@ struct EpiPoly {
       const float dl = pre.dl;
       if (cb + 1 < BN / 64) fetch(p, t, at, row0, n0 + 32, pre);
       float v[32], dg = 0.f;
-      acc_ld32<1, 0>(at.ok, tm + c, v, 1);
+      tmem_ld32(tm + c, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         const float aa = v[j] * (1.f / (kXScale * kXScale));
@@ -135,6 +151,13 @@ struct EpiUpdate {
     float a;
   };
   struct Pre { uint4 h[4], l[4]; float bl; };  // 32 columns of X (rows are padded to 8), diag(B)
+  static __device__ __forceinline__ void poison(const Params& p, const Tiles& t, const TileAt& at, int row0, int half) {
+    const int n0 = at.n * BN + half * (BN / 2);
+    if (p.out != nullptr)
+      fill_nan(p.out + at.batch * p.out_stride + (int64_t)row0 * t.N + n0, t.N, t.M - row0, t.N - n0, BN / 2);
+    else  // the remainders need none: what reads them reads the values too
+      fill_nan(p.x_out + at.batch * p.stride + (int64_t)row0 * p.ld + n0, p.ld, t.M - row0, t.N - n0, BN / 2);
+  }
   static __device__ __forceinline__ void fetch(const Params& p, const Tiles& t, const TileAt& at, int row0, int n0, Pre& pre) {
     const int lane = threadIdx.x & 31;
     const int64_t off = at.batch * p.stride + (int64_t)row0 * p.ld + n0;
@@ -163,7 +186,7 @@ struct EpiUpdate {
       const float bl = pre.bl;
       if (cb + 1 < BN / 64) fetch(p, t, at, row0, n0 + 32, pre);
       float v[32];
-      acc_ld32<1, 0>(at.ok, tm + c, v, 1);
+      tmem_ld32(tm + c, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) {  // 2^12 X
         const float h = __half2float(reinterpret_cast<const __half*>(h4)[j]), l = __half2float(reinterpret_cast<const __half*>(l4)[j]);

@@ -675,5 +675,47 @@ void run_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cudaS
   }
 }
 
+// out = base (0 if null) + the sum over splits of partial [splits][n], in order.  `base` may be `out`.
+template <typename T>
+__global__ void __launch_bounds__(256) split_sum_kernel(const float* __restrict__ partial, int splits, int64_t stride, int64_t n, const float* base, T* out) {
+  chain_wait();
+  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  float s = base != nullptr ? base[i] : 0.f;
+  for (int k = 0; k < splits; ++k) s += partial[k * stride + i];
+  out[i] = narrow<T>(s);
+}
+
+// The product of t's segments into `out` [batches][M][N] with the contraction axis split over `splits` tiles of every output
+// tile: partial sums in memory, added in order.  More than kPartials are formed and added in several rounds.
+constexpr int kPartials = 64;
+template <typename T, int BN, int ACC>
+void split_product(const Maps& maps, Tiles& t, int64_t M, int64_t N, int64_t batches, int splits, bool pair, T* out,
+                   const at::TensorOptions& fp32, cudaStream_t st) {
+  const int64_t n = batches * M * N;
+  at::Tensor part = at::empty({std::min(splits, kPartials), n}, fp32), total;
+  float* sum = nullptr;
+  if (splits > kPartials) {
+    if constexpr (sizeof(T) == 4) {
+      sum = out;
+    } else {
+      total = at::empty({n}, fp32);
+      sum = total.data_ptr<float>();
+    }
+  }
+  const dim3 grid((unsigned)((n + 255) / 256));
+  for (int s0 = 0; s0 < splits; s0 += kPartials) {
+    const int here = std::min(kPartials, splits - s0);
+    set_tiles(t, M, N, BN, batches, here, false, pair);
+    t.splits = splits;
+    t.split0 = s0;
+    typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n, 1.f};
+    run_dense<BN, EpiStore<float, BN, ACC>>(maps, t, ep, st);
+    const float* const base = s0 > 0 ? sum : nullptr;
+    if (s0 + here < splits) launch_chained(split_sum_kernel<float>, grid, 256, st, part.data_ptr<float>(), here, n, n, base, sum);
+    else launch_chained(split_sum_kernel<T>, grid, 256, st, part.data_ptr<float>(), here, n, n, base, out);
+  }
+}
+
 }  // namespace dense
 }  // namespace nva

@@ -285,17 +285,6 @@ void run_packs(const PackJobs& jobs, int planes, cudaStream_t st) {
   launch_chained(planes == 3 ? pack_kernel<float, 3> : pack_kernel<__half, 1>, grid, 256, st, jobs);
 }
 
-// out = base (0 if null) + the sum over splits of partial [splits][n], in order.  `base` may be `out`.
-template <typename T>
-__global__ void split_sum_kernel(const float* __restrict__ partial, int splits, int64_t stride, int64_t n, const float* base, T* out) {
-  chain_wait();
-  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  float s = base != nullptr ? base[i] : 0.f;
-  for (int k = 0; k < splits; ++k) s += partial[k * stride + i];
-  out[i] = narrow<T>(s);
-}
-
 // A matrix as a product reads it.  `mn` says whether the axis that is not contracted is contiguous, when the contraction
 // runs over axis `k_axis` of the logical matrix.
 struct Operand {
@@ -386,8 +375,7 @@ struct Plan {
 
 // Plain product into `out` [batches][M][N].  The contraction axis is split over several tiles (partials added in order by a
 // second kernel) when half of the GPU or more would have no tile and the axis is long, and so that no accumulator takes more
-// than max_blocks.  More than kPartials partials are formed and added in several rounds.
-constexpr int kPartials = 64;
+// than max_blocks.
 template <typename T, int BN, int ACC>
 void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N, cudaStream_t st) {
   set_tiles(pl.t, M, N, BN, batches, 1);
@@ -398,28 +386,12 @@ void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N,
   int splits = 1;
   if (2 * tiles <= at_once) splits = std::max(1, std::min({at_once / tiles, kb / 8, nk, kPartials}));
   splits = std::min(nk, std::max(splits, (load + limit - 1) / limit));
-  if (splits == 1) {
-    typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
-    run_dense<BN, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);
+  if (splits > 1) {
+    split_product<T, BN, ACC>(pl.maps, pl.t, M, N, batches, splits, true, (T*)out.data_ptr(), out.options().dtype(at::kFloat), st);
     return;
   }
-  const int64_t n = batches * M * N;
-  Tensor part = at::empty({std::min(splits, kPartials), n}, out.options().dtype(at::kFloat)), total;
-  if (splits > kPartials) total = sizeof(T) == 4 ? out : at::empty({n}, part.options());
-  const dim3 grid((unsigned)((n + 255) / 256));
-  for (int s0 = 0; s0 < splits; s0 += kPartials) {
-    const int here = std::min(kPartials, splits - s0);
-    set_tiles(pl.t, M, N, BN, batches, here);
-    pl.t.splits = splits;
-    pl.t.split0 = s0;
-    typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n, 1.f};
-    run_dense<BN, EpiStore<float, BN, ACC>>(pl.maps, pl.t, ep, st);
-    const float* const base = s0 > 0 ? total.data_ptr<float>() : nullptr;
-    if (s0 + here < splits)
-      launch_chained(split_sum_kernel<float>, grid, 256, st, part.data_ptr<float>(), here, n, n, base, total.data_ptr<float>());
-    else
-      launch_chained(split_sum_kernel<T>, grid, 256, st, part.data_ptr<float>(), here, n, n, base, (T*)out.data_ptr());
-  }
+  typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
+  run_dense<BN, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);
 }
 
 // Columns of a tile of an M x N product over `kb` blocks of the contraction axis (all segments): by the number of tiles, and 256

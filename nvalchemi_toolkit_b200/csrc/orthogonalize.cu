@@ -515,6 +515,21 @@ void run_small(const Tensor& g, int64_t steps, double a, double b, double c, dou
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+// R and the diagonal of A from a [batch][r][r], the sums of 2^24 A (matrices whose long side is formed in parts).
+__global__ void __launch_bounds__(256) ns_gram_kernel(const float* __restrict__ a, int64_t batch, int r, int ld, __half* __restrict__ out,
+                                                      float* __restrict__ diag) {
+  chain_wait();
+  const int64_t total = batch * r * r;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / r;  // of the batch's rows
+    const int c = (int)(i - row * r);
+    const float v = a[i] * (1.f / kXScale);
+    const bool on = row % r == c;
+    out[row * ld + c] = __float2half_rn(on ? 0.f : v);
+    if (on) diag[row] = v * (1.f / kXScale);
+  }
+}
+
 // Adds a segment: planes za, zb of batch-many matrices each.
 void add_segment(Tiles& t, int a, bool a_mn, int b, bool b_mn, int64_t K, int n, int za = 0, int zb = 0) {
   Seg& s = t.seg[t.n_seg++];
@@ -592,6 +607,14 @@ Tensor newton_schulz(const Tensor& g, int64_t steps, double a, double b, double 
       put_map(maps, 0, stored_x(cur));
       for (int k = two ? 0 : 2; k < 3; ++k)  // remainder . high, high . remainder, high . high
         add_segment(t, 0, tall, 0, tall, tall ? m : n, BN, k == 0 ? (int)batch : 0, k == 1 ? (int)batch : 0);
+      const int load = t.main_nk[0] * t.n_seg, most = max_blocks(at::kBFloat16);  // of the diagonal's sums, all of one sign
+      if (load > most) {
+        Tensor sums = at::empty({batch, r, r}, opt(at::kFloat));
+        split_product<float, BN, 1>(maps, t, r, r, batch, (load + most - 1) / most, gram.pair, sums.data_ptr<float>(), sums.options(), st);
+        launch_chained(ns_gram_kernel, dim3((unsigned)std::min<int64_t>((batch * r * r + 255) / 256, 148 * 8)), 256, st, sums.data_ptr<float>(),
+                       batch, (int)r, (int)rld, rp, ad);
+        return;
+      }
       set_tiles(t, r, r, BN, batch, 1, gram.lower, gram.pair);
       run_dense<BN, EpiGram<BN>>(maps, t, {rp, ad, rld, r * rld}, st);
     });

@@ -215,6 +215,12 @@ struct EpiUpdate {
   }
 };
 
+// 2^12 / (|G| + eps) from the sum of squares; a zero matrix stays zero without eps too.
+__device__ __forceinline__ double scale_of(double squares, double eps) {
+  const double norm = sqrt(squares) + eps;
+  return norm == 0.0 ? 0.0 : (double)kXScale / norm;
+}
+
 // Eight elements at a time where G's rows allow 16-byte accesses (8 | n, aligned), else one by one.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, bool vec, int left, double (&v)[8]) {
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(256) ns_init_kernel(const T* __restrict__ g, i
     double s = 0.0;
     for (int i = threadIdx.x; i < parts; i += 32) s += partial[blockIdx.y * parts + i];
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) scale = (double)kXScale / (sqrt(s) + eps);
+    if (threadIdx.x == 0) scale = scale_of(s, eps);
   }
   __syncthreads();
   const double k = scale;
@@ -346,7 +352,7 @@ __global__ void __launch_bounds__(kSmallThreads)
   for (int i = 0; i < 8; ++i) s += part[i];
   // 2^12 / (|G| + eps) as a mantissa and two powers of two, so that no factor leaves the fp32 range
   int e;
-  const float mant = (float)frexp((double)kXScale / (sqrt(s) + eps), &e);
+  const float mant = (float)frexp(scale_of(s, eps), &e);
   const float p1 = scalbnf(1.f, max(-126, min(127, e / 2))), p2 = scalbnf(1.f, max(-126, min(127, e - e / 2)));
   const uint32_t magic = n > 1 ? (uint32_t)((0x100000000ull + n - 1) / n) : 0;  // i / n = umulhi(i, magic) for i < 2^16, n <= 256
   auto place = [&](uint32_t i) {

@@ -71,8 +71,8 @@ def _formula(x: torch.Tensor, steps: int, a: float, b: float, c: float, eps: flo
     tall = x.shape[-2] > x.shape[-1]
     if tall:
         x = x.transpose(-2, -1)
-    norm = x.double().square().sum((-2, -1), keepdim=True).sqrt()
-    x = (x / (norm + eps)).float()
+    norm = x.double().square().sum((-2, -1), keepdim=True).sqrt() + eps
+    x = (x / torch.where(norm == 0, 1.0, norm)).float()  # a zero matrix stays zero without eps too
     for _ in range(steps):
         gram = x @ x.transpose(-2, -1)
         x = a * x + (b * gram + c * (gram @ gram)) @ x

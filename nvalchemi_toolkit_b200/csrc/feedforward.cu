@@ -25,6 +25,7 @@
 // tile that forms dh.  Narrow blocks (131,072 x 128 -> 512 -> 128) are bound by the epilogue and by h going through memory:
 // 77 us for h, 33 us for y.  float32 (4096 x 256 -> 1024 -> 256) does six times the products: 264 us forward and backward.
 #include "dense16.cuh"
+#include "gate.cuh"
 
 namespace nva {
 using at::Tensor;
@@ -34,53 +35,6 @@ bool gated_ff_rows(const Tensor& x, const Tensor& wg, const Tensor& wu, const Te
 
 namespace {
 using namespace dense;
-
-enum Act : int { kSilu = 0, kGelu = 1 };
-
-// 2^x and 1 / x by the special function unit, one instruction each (subnormal results become 0; 2 and 1 ulp): the epilogues
-// below are bound by what they issue.
-__device__ __forceinline__ float fast_exp2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float fast_rcp(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-constexpr float kLog2e = 1.4426950408889634f;
-
-// The same to fp32 accuracy, without branches.  e^x = 2^t e^(d ln 2) with t = x log2(e) rounded and d what the rounding left;
-// one Newton step for the reciprocal.
-__device__ __forceinline__ float exp32(float x) {
-  x = fminf(fmaxf(x, -87.f), 87.f);
-  const float t = x * kLog2e, d = fmaf(x, kLog2e, -t) + x * 1.925963033e-8f;  // log2(e) - kLog2e
-  return fast_exp2(t) * fmaf(d, 0.69314718f, 1.f);
-}
-__device__ __forceinline__ float rcp32(float x) {
-  const float r = fast_rcp(x);
-  return fmaf(r, fmaf(-x, r, 1.f), r);
-}
-
-// act(g) and act'(g); EXACT: for float32 results, else with the fast functions (1e-6 relative).
-template <bool EXACT, int ACT>
-__device__ __forceinline__ void activate(float g, float& a, float& da) {
-  if constexpr (ACT == kSilu) {
-    const float e = EXACT ? exp32(-g) : fast_exp2(-kLog2e * g), s = EXACT ? rcp32(1.f + e) : fast_rcp(1.f + e);
-    a = g * s;
-    da = s * (1.f + g * (1.f - s));
-  } else {  // g * Phi(g)
-    // erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), z >= 0: Hastings' approximation (Abramowitz and Stegun,
-    // 7.1.26), off by at most 1.5e-7; its exponential is the derivative's as well
-    const float z = 0.70710678118654752f * fabsf(g), q0 = 1.f + 0.3275911f * z;
-    const float e = EXACT ? exp32(-0.5f * g * g) : fast_exp2(-0.5f * kLog2e * g * g), t = EXACT ? rcp32(q0) : fast_rcp(q0);
-    const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-    const float cdf = g < 0.f ? q : 1.f - q;
-    a = g * cdf;
-    da = cdf + g * 0.39894228040143268f * e;
-  }
-}
 
 // The branch on the activation stays outside the loop over a thread's values: inside it the values' chains of dependent
 // instructions would run one after the other (131,072 x 128 x 512: 222 us that way).

@@ -10,6 +10,7 @@
 // time; the second four find the weights in the L2.
 #include "common.cuh"
 #include "convert.cuh"
+#include "gate.cuh"
 
 #include <cooperative_groups.h>
 
@@ -23,8 +24,11 @@ constexpr int kMaxSmem = 96 * 1024, kLanes = 8;  // column lanes of a block
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Vec { T v[VEC]; };
 
-__device__ __forceinline__ float gate_of(int act, float g) {  // 0 silu, 1 gelu
-  return act == 0 ? g / (1.f + expf(-g)) : 0.5f * g * erfcf(-0.70710678118654752f * g);
+__device__ __forceinline__ float gate_of(int act, float g) {
+  float a, da;
+  if (act == kSilu) activate<true, kSilu>(g, a, da);
+  else activate<true, kGelu>(g, a, da);
+  return a;
 }
 
 // x [rows][k0, k1) to shared memory as fp32 [k][R] (one load per k for all rows)

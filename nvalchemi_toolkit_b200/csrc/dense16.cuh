@@ -252,14 +252,19 @@ __device__ __forceinline__ void pack32(const float (&v)[32], uint4 (&o)[Slots<T>
   }
 }
 
-// A float32 value as the exact sum of three bf16 values (8 + 8 + 8 bits), cut off towards zero, so that none passes the value.
-// Without branches: 32 of these run side by side.  Infinities stay in the first part alone.
-__device__ __forceinline__ float cut16(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
-__device__ __forceinline__ void split3(float v, float& p0, float& p1, float& p2) {
-  p0 = cut16(v);
-  const float r = p0 == v ? 0.f : v - p0;
-  p1 = cut16(r);
-  p2 = r - p1;
+// Two float32 values as exact sums of three bf16 values each, p[i] holding the i-th parts (the first value's in the low half).
+// The parts are rounded to nearest: what a product of two values leaves out (second times third parts, third times third) is then
+// at most 2^-24 of it and of either sign, against 2^-21 of one sign for parts cut off towards zero.  Without branches: 16 of these
+// run side by side.  First parts of values past the largest bf16 number are held at it; infinities and NaN are in the other two.
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&p)[3]) {
+  constexpr float kTop = 3.3895313e38f;  // the largest bf16 number
+  p[0] = pack2(fminf(fmaxf(a, -kTop), kTop), fminf(fmaxf(b, -kTop), kTop), __nv_bfloat16{});
+#pragma unroll
+  for (int i = 1; i < 3; ++i) {
+    a -= __uint_as_float(p[i - 1] << 16);
+    b -= __uint_as_float(p[i - 1] & 0xffff0000u);
+    p[i] = pack2(a, b, __nv_bfloat16{});
+  }
 }
 
 // 32 columns of the sum of a group's accumulators, STRIDE columns apart.

@@ -16,7 +16,7 @@
 // dh are formed as float32 matrices by split products and a kernel of its own applies the gate.
 //
 // float32 matrices run on the same tensor cores: a value is the exact sum of three bf16 values and a product the six
-// partial products down to 2^-24; the intermediate h, dg and du are stored as three planes each, so nothing is lost to
+// partial products above 2^-24 of it; the intermediate h, dg and du are stored as three planes each, so nothing is lost to
 // 16 bits.  There dh is a product of its own (its accumulators would not fit beside those of g and u).
 //
 // What bounds it (8192 x 1024 -> 4096 -> 1024, bfloat16): the plain products run at 1150 to 1490 TFLOP/s (51 to 58 us of 69
@@ -64,33 +64,36 @@ __device__ __forceinline__ void gate_grad(float (&g)[C], float (&u)[C], float (&
 template <typename T, int C>
 __device__ __forceinline__ void store_cols(uint4* stage, float (&v)[C], void* dst, int64_t off, int64_t ld, int64_t plane, int rows_left,
                                            int cols_left, int two) {
-  auto put = [&](const float (&f)[C], auto tag, int64_t at) {
-    using S = decltype(tag);
+  using S = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
+  auto put = [&](const uint32_t (&w)[C / 2], int64_t at) {
     uint4 o[C / 8];
 #pragma unroll
-    for (int j = 0; j < C / 8; ++j)
-      o[j] = make_uint4(pack2(f[8 * j], f[8 * j + 1], S{}), pack2(f[8 * j + 2], f[8 * j + 3], S{}), pack2(f[8 * j + 4], f[8 * j + 5], S{}),
-                        pack2(f[8 * j + 6], f[8 * j + 7], S{}));
+    for (int j = 0; j < C / 8; ++j) o[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     store_piece<S, C / 8>(stage, o, (S*)dst + at, ld, rows_left, cols_left, true);  // rows are padded to 8
   };
   if constexpr (sizeof(T) == 2) {
-    put(v, T{}, off);
+    uint32_t w[C / 2];
+#pragma unroll
+    for (int j = 0; j < C / 2; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], T{});
+    put(w, off);
     if (two) {
 #pragma unroll
       for (int j = 0; j < C; ++j) v[j] -= widen(narrow<T>(v[j]));
-      put(v, T{}, off + plane);
+#pragma unroll
+      for (int j = 0; j < C / 2; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], T{});
+      put(w, off + plane);
     }
   } else {
-    float p1[C], p2[C];
+    uint32_t w0[C / 2], w1[C / 2], w2[C / 2];
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      float a, b, c;
-      split3(v[j], a, b, c);
-      v[j] = a; p1[j] = b; p2[j] = c;
+    for (int j = 0; j < C / 2; ++j) {
+      uint32_t p[3];
+      split3(v[2 * j], v[2 * j + 1], p);
+      w0[j] = p[0]; w1[j] = p[1]; w2[j] = p[2];
     }
-    put(v, __nv_bfloat16{}, off);
-    put(p1, __nv_bfloat16{}, off + plane);
-    put(p2, __nv_bfloat16{}, off + 2 * plane);
+    put(w0, off);
+    put(w1, off + plane);
+    put(w2, off + 2 * plane);
   }
 }
 
@@ -222,11 +225,10 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJ
       const uint16_t* s16 = reinterpret_cast<const uint16_t*>(s);
       *reinterpret_cast<uint32_t*>(d) = (uint32_t)s16[0] | (two ? (uint32_t)s16[1] << 16 : 0u);
     } else {
-      float a[3], b[3] = {0.f, 0.f, 0.f};
-      split3((float)s[0], a[0], a[1], a[2]);
-      if (two) split3((float)s[1], b[0], b[1], b[2]);
+      uint32_t p[3];
+      split3((float)s[0], two ? (float)s[1] : 0.f, p);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(d + k * job.plane) = pack2(a[k], b[k], __nv_bfloat16{});
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(d + k * job.plane) = p[k];
     }
   }
 }
@@ -317,7 +319,7 @@ struct Plan {
       s.idesc = idesc16(bf16, s.a_mn, s.b_mn, n, BM);
       if (main) t.main_nk[group] = s.nk;
     };
-    if (oa.planes == 3 && ob.planes == 3) {  // what is left out is below 2^-24
+    if (oa.planes == 3 && ob.planes == 3) {  // what is left out is at most 2^-24 of a product
       add(2, 0); add(0, 2); add(1, 1); add(1, 0); add(0, 1);
     } else {
       if (oa.planes == 2) add(1, 0);
@@ -393,10 +395,10 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ gm,
   chain_wait();
   auto put = [&](void* dst, int64_t at, float v) {
     if constexpr (EXACT) {
-      float p[3];
-      split3(v, p[0], p[1], p[2]);
+      uint32_t p[3];
+      split3(v, 0.f, p);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) ((__nv_bfloat16*)dst)[at + k * out.plane] = __float2bfloat16_rn(p[k]);
+      for (int k = 0; k < 3; ++k) ((__nv_bfloat16*)dst)[at + k * out.plane] = __ushort_as_bfloat16((unsigned short)p[k]);
     } else {
       ((T*)dst)[at] = narrow<T>(v);
       if (out.two) ((T*)dst)[at + out.plane] = narrow<T>(v - widen(narrow<T>(v)));

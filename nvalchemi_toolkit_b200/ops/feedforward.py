@@ -153,10 +153,10 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
                        ) -> torch.Tensor:
     """``(act(x @ w_gate) * (x @ w_up)) @ w_down`` for ``x [..., K]``, ``w_gate`` and ``w_up`` ``[K, H]``, ``w_down [H, N]``;
     ``activation`` is ``"silu"`` or ``"gelu"``.  Differentiable (twice and more).  Under ``torch.autocast`` the arguments are
-    cast to its type first, as those of a matrix product are."""
+    cast to its type first, as those of a matrix product are: floating types but float64."""
     if torch.is_autocast_enabled(x.device.type):
         dt = torch.get_autocast_dtype(x.device.type)
-        x, w_gate, w_up, w_down = (t.to(dt) for t in (x, w_gate, w_up, w_down))
+        x, w_gate, w_up, w_down = (t.to(dt) if t.is_floating_point() and t.dtype != torch.float64 else t for t in (x, w_gate, w_up, w_down))
     if not x.is_cuda:
         _check(x, w_gate, w_up, w_down, activation)
         return _forward_formula(x, w_gate, w_up, w_down, activation)

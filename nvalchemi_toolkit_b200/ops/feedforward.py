@@ -48,6 +48,38 @@ def _wide(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.float64 else t.float()
 
 
+class _Product(torch.autograd.Function):
+    """``a @ b`` in the type of its arguments inside an autocast region too, and so are its derivatives."""
+
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(a, b):
+        with torch.autocast(a.device.type, enabled=False):
+            return a @ b
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(*inputs)
+        ctx.save_for_forward(*inputs)
+
+    @staticmethod
+    def backward(ctx, grad):
+        a, b = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return _Product.apply(grad, b.mT) if need[0] else None, _Product.apply(a.mT, grad) if need[1] else None
+
+    @staticmethod
+    def jvp(ctx, da, db):
+        a, b = ctx.saved_tensors
+        terms = [_Product.apply(*t) for t in ((da, b), (a, db)) if t[0] is not None and t[1] is not None]
+        return sum(terms[1:], terms[0])
+
+
+def _product(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    return _Product.apply(a, b) if torch.is_autocast_enabled(a.device.type) else a @ b
+
+
 def _activate(g: torch.Tensor, activation: str) -> tuple[torch.Tensor, torch.Tensor]:
     """``act(g)`` and ``act'(g)``, both differentiable."""
     if activation == "silu":
@@ -59,18 +91,18 @@ def _activate(g: torch.Tensor, activation: str) -> tuple[torch.Tensor, torch.Ten
 
 def _forward_formula(x, w_gate, w_up, w_down, activation):
     xf = _wide(x)
-    h = _activate(xf @ _wide(w_gate), activation)[0] * (xf @ _wide(w_up))
-    return (h @ _wide(w_down)).to(x.dtype)
+    h = _activate(_product(xf, _wide(w_gate)), activation)[0] * _product(xf, _wide(w_up))
+    return _product(h, _wide(w_down)).to(x.dtype)
 
 
 def _backward_formula(dy, x, w_gate, w_up, w_down, activation):
     """``(dx, dw_gate, dw_up, dw_down)`` in differentiable operations, at least 32 bits wide; matrices only."""
     dy, x, wg, wu, wd = (_wide(t) for t in (dy, x, w_gate, w_up, w_down))
-    u = x @ wu
-    a, da = _activate(x @ wg, activation)
-    dh = dy @ wd.t()
+    u = _product(x, wu)
+    a, da = _activate(_product(x, wg), activation)
+    dh = _product(dy, wd.t())
     dg, du = dh * u * da, dh * a
-    return dg @ wg.t() + du @ wu.t(), x.t() @ dg, x.t() @ du, (a * u).t() @ dy
+    return _product(dg, wg.t()) + _product(du, wu.t()), _product(x.t(), dg), _product(x.t(), du), _product((a * u).t(), dy)
 
 
 def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,

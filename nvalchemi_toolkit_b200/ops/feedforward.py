@@ -95,14 +95,16 @@ def _forward_formula(x, w_gate, w_up, w_down, activation):
     return _product(h, _wide(w_down)).to(x.dtype)
 
 
-def _backward_formula(dy, x, w_gate, w_up, w_down, activation):
-    """``(dx, dw_gate, dw_up, dw_down)`` in differentiable operations, at least 32 bits wide; matrices only."""
+def _backward_formula(dy, x, w_gate, w_up, w_down, activation, want=(True,) * 4):
+    """``(dx, dw_gate, dw_up, dw_down)`` in differentiable operations, at least 32 bits wide; matrices only.  ``None`` where
+    ``want`` says so."""
     dy, x, wg, wu, wd = (_wide(t) for t in (dy, x, w_gate, w_up, w_down))
     u = _product(x, wu)
     a, da = _activate(_product(x, wg), activation)
     dh = _product(dy, wd.t())
     dg, du = dh * u * da, dh * a
-    return _product(dg, wg.t()) + _product(du, wu.t()), _product(x.t(), dg), _product(x.t(), du), _product((a * u).t(), dy)
+    return (_product(dg, wg.t()) + _product(du, wu.t()) if want[0] else None, _product(x.t(), dg) if want[1] else None,
+            _product(x.t(), du) if want[2] else None, _product((a * u).t(), dy) if want[3] else None)
 
 
 def gated_feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
@@ -161,6 +163,7 @@ class _GatedFeedForwardGrad(torch.autograd.Function):
     @staticmethod
     def forward(ctx, dy, x, w_gate, w_up, w_down, activation, input_grad, weight_grads):
         ctx.save_for_backward(dy, x, w_gate, w_up, w_down)
+        ctx.set_materialize_grads(False)  # None, not zeros, for the gradients that were not used
         ctx.activation = activation
         return gated_feed_forward_backward(dy, x, w_gate, w_up, w_down, activation, input_grad=input_grad, weight_grads=weight_grads)
 
@@ -171,8 +174,9 @@ class _GatedFeedForwardGrad(torch.autograd.Function):
         with torch.enable_grad():
             args = [t if again else t.detach().requires_grad_(n) for t, n in zip(saved, need)]
             dy, x = args[:2]
-            dx, *dw = _backward_formula(dy.reshape(-1, dy.shape[-1]), x.reshape(-1, x.shape[-1]), *args[2:], ctx.activation)
-            outs = (dx.reshape(x.shape), *dw)
+            dx, *dw = _backward_formula(dy.reshape(-1, dy.shape[-1]), x.reshape(-1, x.shape[-1]), *args[2:], ctx.activation,
+                                        [d is not None for d in dd])
+            outs = (None if dx is None else dx.reshape(x.shape), *dw)
             pairs = [(o, d) for o, d in zip(outs, dd) if d is not None and o.requires_grad]
             wanted = [t for t, n in zip(args, need) if n]
             got = torch.autograd.grad([o for o, _ in pairs], wanted, [d.to(o.dtype) for o, d in pairs], create_graph=again,

@@ -56,16 +56,18 @@ def _forward_formula(x, weight, bias, eps):
     return y.to(x.dtype), mean.reshape(-1), rstd.reshape(-1)
 
 
-def _backward_formula(grad, x, weight, eps):
-    """``(dx, dweight, dbias)`` from ``grad`` and ``x`` in differentiable operations, in at least 32 bits."""
+def _backward_formula(grad, x, weight, eps, want=(True,) * 3):
+    """``(dx, dweight, dbias)`` from ``grad`` and ``x`` in differentiable operations, in at least 32 bits.  ``None`` where ``want``
+    says so."""
     xf, g = _wide(x), _wide(grad)
     d = xf - xf.mean(-1, keepdim=True)
     rstd = torch.rsqrt((d * d).mean(-1, keepdim=True) + eps)
     xh = d * rstd
-    gw = g if weight is None else g * _wide(weight)
-    dx = rstd * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
-    n = x.shape[-1]
-    return dx, (g * xh).reshape(-1, n).sum(0), g.reshape(-1, n).sum(0)
+    dx, n = None, x.shape[-1]
+    if want[0]:
+        gw = g if weight is None else g * _wide(weight)
+        dx = rstd * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))
+    return dx, (g * xh).reshape(-1, n).sum(0) if want[1] else None, g.reshape(-1, n).sum(0) if want[2] else None
 
 
 def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -144,6 +146,7 @@ class _LayerNormGrad(torch.autograd.Function):
     @staticmethod
     def forward(ctx, grad, x, weight, bias, mean, rstd, eps, param_grads):
         ctx.save_for_backward(grad, x, weight)
+        ctx.set_materialize_grads(False)  # None, not zeros, for the gradients that were not used
         ctx.eps, ctx.param_grads = eps, param_grads
         ptype = None if weight is not None or bias is None else bias.dtype
         dx, dw, db = layer_norm_backward(grad, x, mean, rstd, weight, param_grads=param_grads, param_dtype=ptype)
@@ -156,7 +159,7 @@ class _LayerNormGrad(torch.autograd.Function):
         again = torch.is_grad_enabled()  # a third derivative is wanted: keep the graph of this one
         with torch.enable_grad():
             args = [t if t is None or again else t.detach().requires_grad_(n) for t, n in zip(saved, need)]
-            outs = _backward_formula(*args, ctx.eps)
+            outs = _backward_formula(*args, ctx.eps, tuple(d is not None for d in (ddx, ddw, ddb)))
             pairs = [(o, d) for o, d in zip(outs, (ddx, ddw, ddb)) if d is not None and o.requires_grad]
             wanted = [t for t, n in zip(args, need) if n]
             got = torch.autograd.grad([o for o, _ in pairs], wanted, [d.to(o.dtype) for o, d in pairs], create_graph=again,

@@ -23,15 +23,6 @@ __device__ __forceinline__ float fast_rcp(float x) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// c[0] + c[1] t + ... + c[N - 1] t^(N - 1)
-template <int N>
-__device__ __forceinline__ float poly(const float (&c)[N], float t) {
-  float r = c[N - 1];
-#pragma unroll
-  for (int i = N - 2; i >= 0; --i) r = fmaf(r, t, c[i]);
-  return r;
-}
-
 // act(g) and act'(g).  EXACT, for float32 results: a few 2^-24 of the value at every g (silu 5, gelu 8 with its tail; the
 // derivatives of the sum of their terms' magnitudes), without branches, so that a thread's values run side by side.  Else with
 // the fast functions, 3e-6 of the value, which is little beside half a step of 16 bits.  Infinities give NaN or infinity.
@@ -50,20 +41,22 @@ __device__ __forceinline__ void activate(float g, float& a, float& da) {
     // (reweighted least squares on 4000 points) over |g| <= 16, where the exponential has long left the fp32 range; 4.4e-8 with
     // nine coefficients, 1.8e-6 with seven.  Relative, because act(g) of a negative g is all tail.  Its exponential is the
     // derivative's as well.
-    const float z = fminf(fabsf(g), 16.f), d = fmaf(0.35355339059327376f, z, 1.f);
     float e, q;
     if constexpr (EXACT) {
       constexpr float c[9] = {0.141042367f, 0.14120248f, 0.121443897f, 0.101771072f, -0.0143238446f, 0.140501097f, -0.244882271f,
                               0.142906472f, -0.0296612736f};
-      const float h = z * z, low = fmaf(z, z, -h), t = __fdividef(1.f, d);
+      const float z = fminf(fabsf(g), 16.f), h = z * z, low = fmaf(z, z, -h), t = __fdividef(1.f, fmaf(0.35355339059327376f, z, 1.f));
       e = expf(-0.5f * h);
       e = fmaf(-0.5f * low, e, e);  // what rounding the square left
-      q = e * t * poly(c, t);
+      float p = c[8];
+#pragma unroll
+      for (int i = 7; i >= 0; --i) p = fmaf(p, t, c[i]);
+      q = e * t * p;
     } else {
-      constexpr float c[7] = {0.141146347f, 0.139064237f, 0.139263988f, 0.0229727123f, 0.18885614f, -0.174219206f, 0.0429148637f};
-      const float t = fast_rcp(d);
-      e = fast_exp2(-0.5f * kLog2e * z * z);
-      q = e * t * poly(c, t);
+      const float t = fast_rcp(1.f + 0.35355339059327376f * fabsf(g));
+      e = fast_exp2(-0.5f * kLog2e * g * g);
+      q = e * t * (0.141146347f + t * (0.139064237f + t * (0.139263988f + t * (0.0229727123f + t * (0.18885614f +
+          t * (-0.174219206f + t * 0.0429148637f))))));
     }
     const float cdf = g < 0.f ? q : 1.f - q;
     a = g * cdf;

@@ -592,8 +592,9 @@ int64_t gated_ff_error_status(const Tensor& like) { return dense::take_error(lik
 
 }  // namespace nva
 
+// Explicit kernels: tracing must not decompose them, their C++ would launch on tensors without memory.
 TORCH_LIBRARY_FRAGMENT(nvalchemi, m) {
-  m.def("gated_ff_fwd(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> Tensor", &nva::gated_ff_fwd);
-  m.def("gated_ff_bwd(Tensor dy, Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act, int which) -> (Tensor, Tensor, Tensor, Tensor)", &nva::gated_ff_bwd);
-  m.def("gated_ff_error_status(Tensor like) -> int", &nva::gated_ff_error_status);
+  m.def("gated_ff_fwd(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act) -> Tensor", torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, &nva::gated_ff_fwd));
+  m.def("gated_ff_bwd(Tensor dy, Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, int act, int which) -> (Tensor, Tensor, Tensor, Tensor)", torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, &nva::gated_ff_bwd));
+  m.def("gated_ff_error_status(Tensor like) -> int", torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, &nva::gated_ff_error_status));
 }

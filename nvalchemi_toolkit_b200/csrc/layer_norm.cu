@@ -477,8 +477,9 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad, const Tens
 
 }  // namespace nva
 
+// Explicit kernels: tracing must not decompose them, their C++ would launch on tensors without memory.
 TORCH_LIBRARY_FRAGMENT(nvalchemi, m) {
-  m.def("layer_norm_apply(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", &nva::layer_norm_apply);
-  m.def("layer_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)", &nva::layer_norm_fwd);
-  m.def("layer_norm_bwd(Tensor grad, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, bool want_params, ScalarType? param_type) -> (Tensor, Tensor, Tensor)", &nva::layer_norm_bwd);
+  m.def("layer_norm_apply(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, &nva::layer_norm_apply));
+  m.def("layer_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)", torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, &nva::layer_norm_fwd));
+  m.def("layer_norm_bwd(Tensor grad, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, bool want_params, ScalarType? param_type) -> (Tensor, Tensor, Tensor)", torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, &nva::layer_norm_bwd));
 }

@@ -656,7 +656,8 @@ int64_t newton_schulz_error_status(const Tensor& like) { return dense::take_erro
 
 }  // namespace nva
 
+// Explicit kernels: tracing must not decompose them, their C++ would launch on tensors without memory.
 TORCH_LIBRARY_FRAGMENT(nvalchemi, m) {
-  m.def("newton_schulz(Tensor g, int steps, float a, float b, float c, float eps) -> Tensor", &nva::newton_schulz);
-  m.def("newton_schulz_error_status(Tensor like) -> int", &nva::newton_schulz_error_status);
+  m.def("newton_schulz(Tensor g, int steps, float a, float b, float c, float eps) -> Tensor", torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, &nva::newton_schulz));
+  m.def("newton_schulz_error_status(Tensor like) -> int", torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, &nva::newton_schulz_error_status));
 }

@@ -72,7 +72,7 @@ _fakes_done = False
 
 
 def _register_fakes() -> None:
-    """``torch.library.register_fake`` for the operators dynamics code calls, so that a function using them can be traced
+    """``torch.library.register_fake`` for the operators that dynamics code and the dense blocks call, so that a function using them can be traced
     (``torch.compile(fullgraph=True)``, ``make_fx``) without entering the kernels: they become opaque graph nodes, as the
     reference's custom ops are (``nvalchemi/dynamics/_ops/velocity_verlet.py:50-143``).  Runs once, after the library
     has been loaded."""
@@ -91,6 +91,7 @@ def _register_fakes() -> None:
         "momentum_sums": lambda v, m, b, n: v.new_empty(n, 4),
         "wrap_positions": lambda p, *a, **k: torch.empty_like(p),
     }
+    shaped.update(_dense_fakes())
     for name in nothing:
         shaped[name] = lambda *a, **k: None
     for name, fn in shaped.items():
@@ -98,6 +99,39 @@ def _register_fakes() -> None:
             torch.library.register_fake(f"nvalchemi::{name}")(fn)
         except (RuntimeError, ValueError):  # operator absent from an older build of the library
             pass
+
+
+def _dense_fakes() -> dict:
+    """Fakes of layer norm, the gated block and Newton-Schulz; they refuse what the operators refuse."""
+    def stat(x):
+        return x.new_empty(x.numel() // x.shape[-1], dtype=torch.float64 if x.dtype == torch.float64 else torch.float32)
+
+    def layer_norm_apply(x, weight, bias, eps):
+        norm._check(x, weight, bias)
+        return x.new_empty(x.shape)
+
+    def layer_norm_bwd(grad, x, mean, rstd, weight, want_params, param_type):
+        norm._check_backward(grad, x, mean, rstd, weight, param_type)
+        dw = x.new_empty(x.shape[-1] if want_params else 0, dtype=weight.dtype if weight is not None else param_type or x.dtype)
+        return x.new_empty(x.shape), dw, torch.empty_like(dw)
+
+    def gated_ff_fwd(x, w_gate, w_up, w_down, act):
+        feedforward._check(x, w_gate, w_up, w_down, names[act] if act in names else act)
+        return x.new_empty(*x.shape[:-1], w_down.shape[1])
+
+    def gated_ff_bwd(dy, x, w_gate, w_up, w_down, act, which):
+        feedforward._check_backward(dy, x, w_gate, w_up, w_down, names[act] if act in names else act)
+        up = x.new_empty(w_gate.shape[0] if which & 2 else 0, w_gate.shape[1])
+        return (x.new_empty(x.shape if which & 1 else 0), up, torch.empty_like(up),
+                x.new_empty(w_down.shape[0] if which & 4 else 0, w_down.shape[1]))
+
+    from nvalchemi_toolkit_b200.ops import feedforward, norm
+
+    names = {v: k for k, v in feedforward.ACTIVATIONS.items()}
+    return {"layer_norm_apply": layer_norm_apply, "layer_norm_bwd": layer_norm_bwd,
+            "layer_norm_fwd": lambda x, w, b, eps: (layer_norm_apply(x, w, b, eps), stat(x), stat(x)),
+            "gated_ff_fwd": gated_ff_fwd, "gated_ff_bwd": gated_ff_bwd,
+            "newton_schulz": lambda g, *a: g.new_empty(g.shape, dtype=torch.bfloat16)}
 
 
 def available() -> bool:

@@ -51,18 +51,22 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params: Any, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  ns_steps: int = 5, betas: tuple[float, float] = (0.9, 0.999), adam_eps: float = 1e-8, orthogonalize: bool = True) -> None:
-        if not lr >= 0.0:
-            raise ValueError(f"Muon: lr must not be negative, got {lr}")
-        if not 0.0 <= momentum < 1.0:
-            raise ValueError(f"Muon: momentum must lie in [0, 1), got {momentum}")
-        if not weight_decay >= 0.0:
-            raise ValueError(f"Muon: weight_decay must not be negative, got {weight_decay}")
-        if not all(0.0 <= b < 1.0 for b in betas) or not adam_eps > 0.0:
-            raise ValueError(f"Muon: betas must lie in [0, 1) and adam_eps be positive, got {betas}, {adam_eps}")
-        if int(ns_steps) != ns_steps or ns_steps < 1:
-            raise ValueError(f"Muon: ns_steps must be a positive whole number, got {ns_steps}")
-        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=int(ns_steps),
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps,
                                       betas=tuple(betas), adam_eps=adam_eps, orthogonalize=orthogonalize))
+
+    def add_param_group(self, param_group: dict[str, Any]) -> None:
+        o = {**self.defaults, **param_group}
+        if not o["lr"] >= 0.0:
+            raise ValueError(f"Muon: lr must not be negative, got {o['lr']}")
+        if not 0.0 <= o["momentum"] < 1.0:
+            raise ValueError(f"Muon: momentum must lie in [0, 1), got {o['momentum']}")
+        if not o["weight_decay"] >= 0.0:
+            raise ValueError(f"Muon: weight_decay must not be negative, got {o['weight_decay']}")
+        if not all(0.0 <= b < 1.0 for b in o["betas"]) or not o["adam_eps"] > 0.0:
+            raise ValueError(f"Muon: betas must lie in [0, 1) and adam_eps be positive, got {o['betas']}, {o['adam_eps']}")
+        if int(o["ns_steps"]) != o["ns_steps"] or not 1 <= o["ns_steps"] <= 100:
+            raise ValueError(f"Muon: ns_steps must be a whole number in 1..100, got {o['ns_steps']}")
+        super().add_param_group(param_group)
 
     @staticmethod
     def _is_matrix(p: torch.Tensor) -> bool:

@@ -111,3 +111,19 @@ def test_state_survives_a_saved_copy(dtype, device):
     opt.step()
     other.step()
     assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("bad", [dict(ns_steps=101), dict(ns_steps=2.5), dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-0.1),
+                                 dict(betas=(0.9, 1.0)), dict(adam_eps=0.0)])
+def test_refused_before_the_first_step(bad):
+    """What the step could not carry out is refused when the optimiser, or one of its groups, is made."""
+    p, q = (torch.nn.Parameter(torch.randn(4, 4)) for _ in range(2))
+    with pytest.raises(ValueError, match="Muon"):
+        Muon([p], **bad)
+    with pytest.raises(ValueError, match="Muon"):
+        Muon([{"params": [p]}, {"params": [q], **bad}])
+    opt = Muon([p])
+    with pytest.raises(ValueError, match="Muon"):
+        opt.add_param_group({"params": [q], **bad})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": [q], "lr": 0.0, "ns_steps": 100, "orthogonalize": False})

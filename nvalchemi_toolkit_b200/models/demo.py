@@ -35,7 +35,8 @@ class DemoModel(nn.Module):
         z = self.embedding(atomic_numbers.long())
         c = self.coord_embedding(positions)
         h = self.joint_mlp(torch.cat([z, c], dim=-1))
-        return h if self.gated_block is None else self.gated_block(h)
+        block = getattr(self, "gated_block", None)  # absent from objects saved before there was one
+        return h if block is None else block(h)
 
     def forward(self, atomic_numbers: torch.Tensor, positions: torch.Tensor, batch_idx: torch.Tensor,
                 num_graphs: int) -> tuple[torch.Tensor, torch.Tensor]:

@@ -12,5 +12,6 @@ def test_a_model_without_the_attribute_still_runs():
     want = model(data)
     del model.model.gated_block, model.model.gated_hidden     # as an older object comes out of torch.load
     got = model(data)
-    assert all(torch.equal(got[k], want[k]) for k in ("energy", "forces"))
+    # every call scales embeddings of norm 1 back to norm 1, which may move their last bits: a chain of a hundred operations
+    assert all(float((got[k] - want[k]).abs().max()) <= 100 * 2.0 ** -24 * float(want[k].abs().max()) for k in ("energy", "forces"))
     assert model.checkpoint_spec()["config"] == {"hidden_dim": 16}

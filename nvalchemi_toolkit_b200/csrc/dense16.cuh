@@ -492,13 +492,13 @@ struct NoPrefetch {
   static __device__ __forceinline__ void prefetch(const P&, const Tiles&, const TileAt&, int, int, Pre&) {}
 };
 
-// out[batch][split][M][N] = alpha * acc, as T.
+// out[batch][split][M][N] = acc, as T.
 template <typename T, int BN, int ACC>
 struct EpiStore : NoPrefetch {
   static constexpr int kAcc = ACC, kStride = BN;
   static constexpr bool kLate = false;
   static_assert(ACC == 1 || ACC * BN <= 512, "dense: accumulators exceed the TMEM");
-  struct Params { T* out; int64_t ld, batch_stride, split_stride; float alpha; };
+  struct Params { T* out; int64_t ld, batch_stride, split_stride; };
   static __device__ __forceinline__ void poison(const Params& p, const Tiles& t, const TileAt& at, int row0, int part) {
     const int n0 = at.n * BN + part * (BN / 2);
     fill_nan(p.out + at.batch * p.batch_stride + (at.split - t.split0) * p.split_stride + (int64_t)row0 * p.ld + n0, p.ld, t.M - row0,
@@ -515,8 +515,6 @@ struct EpiStore : NoPrefetch {
       const int c = part * COLS + cb * 32, n0 = at.n * BN + c;
       float v[32];
       acc_ld32<ACC, BN>(tm + c, v, used);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= p.alpha;
       uint4 o[Slots<T>::n];
       pack32<T>(v, o);
       store_piece<T, Slots<T>::n>(stage, o, out + (int64_t)row0 * p.ld + n0, p.ld, t.M - row0, t.N - n0, vec_ok);
@@ -664,7 +662,7 @@ void launch_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cu
   cfg.numAttrs = PAIR ? 2 : 1;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, dense_kernel<BN, PAIR, Epi>, maps, t, ep));
 }
-template <int BN, typename Epi, bool PAIR_OK = true>
+template <int BN, typename Epi>
 void run_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cudaStream_t st) {
   if constexpr (BN == 64) {
     launch_dense<BN, false, Epi>(maps, t, ep, st);
@@ -674,7 +672,7 @@ void run_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cudaS
     } else {
       launch_dense<BN, false, Epi>(maps, t, ep, st);
     }
-  } else if constexpr (PAIR_OK) {
+  } else {
     for (int i = 0; i < t.n_seg; ++i) TORCH_CHECK(t.seg[i].n % 128 == 0, "dense: a segment too narrow for a pair");
     launch_dense<BN, true, Epi>(maps, t, ep, st);
   }
@@ -714,7 +712,7 @@ void split_product(const Maps& maps, Tiles& t, int64_t M, int64_t N, int64_t bat
     set_tiles(t, M, N, BN, batches, here, false, pair);
     t.splits = splits;
     t.split0 = s0;
-    typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n, 1.f};
+    typename EpiStore<float, BN, ACC>::Params ep{part.data_ptr<float>(), N, M * N, n};
     run_dense<BN, EpiStore<float, BN, ACC>>(maps, t, ep, st);
     const float* const base = s0 > 0 ? sum : nullptr;
     if (s0 + here < splits) launch_chained(split_sum_kernel<float>, grid, 256, st, part.data_ptr<float>(), here, n, n, base, sum);

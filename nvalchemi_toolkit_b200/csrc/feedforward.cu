@@ -346,7 +346,7 @@ void store_product(Plan& pl, Tensor& out, int64_t batches, int64_t M, int64_t N,
     split_product<T, BN, ACC>(pl.maps, pl.t, M, N, batches, splits, true, (T*)out.data_ptr(), out.options().dtype(at::kFloat), st);
     return;
   }
-  typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0, 1.f};
+  typename EpiStore<T, BN, ACC>::Params ep{(T*)out.data_ptr(), N, M * N, 0};
   run_dense<BN, EpiStore<T, BN, ACC>>(pl.maps, pl.t, ep, st);
 }
 

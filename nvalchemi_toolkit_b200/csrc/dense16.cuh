@@ -690,15 +690,17 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const float* __restrict_
 }
 
 // The product of t's segments into `out` [batches][M][N] with the contraction axis split over `splits` tiles of every output
-// tile: partial sums in memory, added in order.  More than kPartials are formed and added in several rounds.
+// tile: partial sums in memory, added in order.  More than kPartials of them, or more than 1 GB, are formed and added in rounds.
 constexpr int kPartials = 64;
+constexpr int64_t kPartialFloats = 1ll << 28;
 template <typename T, int BN, int ACC>
 void split_product(const Maps& maps, Tiles& t, int64_t M, int64_t N, int64_t batches, int splits, bool pair, T* out,
                    const at::TensorOptions& fp32, cudaStream_t st) {
   const int64_t n = batches * M * N;
-  at::Tensor part = at::empty({std::min(splits, kPartials), n}, fp32), total;
+  const int round = (int)std::max<int64_t>(1, std::min<int64_t>({splits, kPartials, kPartialFloats / n}));
+  at::Tensor part = at::empty({round, n}, fp32), total;
   float* sum = nullptr;
-  if (splits > kPartials) {
+  if (splits > round) {
     if constexpr (sizeof(T) == 4) {
       sum = out;
     } else {
@@ -707,8 +709,8 @@ void split_product(const Maps& maps, Tiles& t, int64_t M, int64_t N, int64_t bat
     }
   }
   const dim3 grid((unsigned)((n + 255) / 256));
-  for (int s0 = 0; s0 < splits; s0 += kPartials) {
-    const int here = std::min(kPartials, splits - s0);
+  for (int s0 = 0; s0 < splits; s0 += round) {
+    const int here = std::min(round, splits - s0);
     set_tiles(t, M, N, BN, batches, here, false, pair);
     t.splits = splits;
     t.split0 = s0;

@@ -58,3 +58,22 @@ def test_wide_projections_float32(width):
 def test_axes_past_the_accumulators(m, k, h, n, dtype, layout, act):
     """Against float64, element by element; only the bounds of `tests/test_feedforward.py`, which count the length, apply here."""
     _run(m, k, h, n, dtype, "cuda", act, layout)
+
+
+def test_partial_sums_take_bounded_memory():
+    """float16 over 262,144 rows splits into 32 parts of 134 MB; beyond h, dg, du (2.1 GB each) and the gradients no more than
+    1.5 GB is held."""
+    x, wg, wu, wd, dy = _positive(262144, 32, 4096, 8192, F16, 2.0 ** -8)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = ff.gated_feed_forward_backward(dy, x, wg, wu, wd)
+    torch.cuda.synchronize()
+    held = torch.cuda.max_memory_allocated() - before - 3 * 262144 * 4096 * 2 - sum(g.numel() * g.element_size() for g in grads)
+    assert held <= 1.5 * 2 ** 30, held / 2 ** 30
+    rows = torch.arange(0, 4096, 512, device="cuda")
+    h = torch.nn.functional.silu(x.double() @ wg[:, rows].double()) * (x.double() @ wu[:, rows].double())
+    want = torch.cat([h.t() @ dy[:, i:i + 1024].double() for i in range(0, 8192, 1024)], 1)
+    mean = float(((grads[3][rows].double() - want) / want).mean())
+    assert abs(mean) <= 2.0 ** -11 * (1 / 8 + 4 / want.numel() ** 0.5)

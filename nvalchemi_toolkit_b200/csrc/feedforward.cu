@@ -374,8 +374,15 @@ void store_any(Plan& pl, int bn, Tensor& out, int64_t batches, int64_t M, int64_
   else go(__nv_bfloat16{});
 }
 
-// Whether a projection over an axis of K is too long for the accumulators of one tile (float32: two of them).
-bool far(const Tensor& x, int64_t K) { return (K + BK - 1) / BK > max_blocks(x.scalar_type()) * (x.scalar_type() == at::kFloat ? 2 : 1); }
+// Whether a projection over an axis of K is too long for the accumulators of one tile (float32: four of them, at most).
+bool far(const Tensor& x, int64_t K) { return (K + BK - 1) / BK > max_blocks(x.scalar_type()) * (x.scalar_type() == at::kFloat ? 4 : 1); }
+
+// Columns (of g and u together) of the tiles that form both projections.  float32: 256 leave room for two accumulators, 128 for
+// four.
+int gate_bn(const Tensor& x, int64_t M, int64_t H, int64_t K) {
+  const bool two = x.scalar_type() != at::kFloat || (K + BK - 1) / BK <= 2 * max_blocks(at::kFloat);
+  return two ? store_bn(1, M, 2 * H, 0) : 128;
+}
 
 // out [M][N] float32 = a . b over axes 1 and `kb`.
 void project(bool bf16, const Operand& a, const Operand& b, int kb, Tensor& out, cudaStream_t st) {
@@ -492,7 +499,7 @@ Tensor gated_ff_fwd(const Tensor& x_in, const Tensor& wg, const Tensor& wu, cons
       run_dense<BN, EpiGated<T, BN>>(pl.maps, pl.t, ep, st);
     };
     auto wide = [&](auto v) {
-      if (store_bn(1, M, 2 * H, 0) == 256) go(v, std::integral_constant<int, 256>{});
+      if (gate_bn(x, M, H, K) == 256) go(v, std::integral_constant<int, 256>{});
       else go(v, std::integral_constant<int, 128>{});
     };
     if (P == 3) wide(float{});
@@ -557,7 +564,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ff_bwd(const Tensor& dy_in, con
         set_tiles(pl.t, M, H, BN / 2, 1, 1);
         run_dense<BN, EpiGatedGradRead<BN>>(pl.maps, pl.t, {out, dh.data_ptr<float>(), ld_dh}, st);
       };
-      if (store_bn(1, M, 2 * H, 0) == 256) go(std::integral_constant<int, 256>{});
+      if (gate_bn(x, M, H, K) == 256) go(std::integral_constant<int, 256>{});
       else go(std::integral_constant<int, 128>{});
     }
   }

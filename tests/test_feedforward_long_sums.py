@@ -52,7 +52,7 @@ def test_wide_projections_float32(width):
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("m,k,h,n,dtype,layout", [
-    (130, 2500, 257, 129, F32, None), (130, 1025, 130, 70, F32, "mixed"), (20, 2049, 40, 24, F32, "linear"), (300, 2100, 33, 2100, F32, "sliced"),
+    (130, 2500, 257, 129, F32, None), (1000, 2000, 257, 129, F32, None), (130, 1025, 130, 70, F32, "mixed"), (20, 2049, 40, 24, F32, "linear"), (300, 2100, 33, 2100, F32, "sliced"),
     (200, 9000, 72, 40, F16, None), (300, 40, 72, 9000, F16, "mixed"), (300, 8200, 65, 8200, F16, "linear"),
     (130, 70000, 64, 16, BF16, None), (20, 16, 64, 70000, BF16, None)])
 def test_axes_past_the_accumulators(m, k, h, n, dtype, layout, act):

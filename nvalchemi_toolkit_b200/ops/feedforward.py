@@ -76,8 +76,13 @@ class _Product(torch.autograd.Function):
         return sum(terms[1:], terms[0])
 
 
+def _in_autocast(t: torch.Tensor) -> bool:
+    kind = t.device.type
+    return (t.is_cuda or torch.amp.is_autocast_available(kind)) and torch.is_autocast_enabled(kind)
+
+
 def _product(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
-    return _Product.apply(a, b) if torch.is_autocast_enabled(a.device.type) else a @ b
+    return _Product.apply(a, b) if _in_autocast(a) else a @ b
 
 
 def _activate(g: torch.Tensor, activation: str) -> tuple[torch.Tensor, torch.Tensor]:
@@ -190,7 +195,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     """``(act(x @ w_gate) * (x @ w_up)) @ w_down`` for ``x [..., K]``, ``w_gate`` and ``w_up`` ``[K, H]``, ``w_down [H, N]``;
     ``activation`` is ``"silu"`` or ``"gelu"``.  Differentiable (twice and more).  Under ``torch.autocast`` the arguments are
     cast to its type first, as those of a matrix product are: floating types but float64."""
-    if torch.is_autocast_enabled(x.device.type):
+    if _in_autocast(x):
         dt = torch.get_autocast_dtype(x.device.type)
         x, w_gate, w_up, w_down = (t.to(dt) if t.is_floating_point() and t.dtype != torch.float64 else t for t in (x, w_gate, w_up, w_down))
     if not x.is_cuda:

@@ -67,3 +67,15 @@ def test_force_training_inside_autocast(device):
     want = _force_step([t.double().cpu() for t in ts], torch.autocast("cpu", enabled=False))
     for a, b in zip(got, want):
         assert float(((a.double().cpu() - b).norm() / b.norm()).detach()) < 8 * 2.0 ** -8
+
+
+def test_devices_without_autocast():
+    """Shapes of a model on the meta device, as they are asked for before weights are loaded."""
+    from nvalchemi_toolkit_b200.models import GatedBlock
+
+    with torch.device("meta"):
+        block = GatedBlock(8, 12)
+        x = torch.empty(3, 8, requires_grad=True)
+    y = block(x)
+    assert y.shape == (3, 8) and y.device.type == "meta"
+    assert [g.shape for g in torch.autograd.grad(y.sum(), [x, block.feed_forward.w_down])] == [(3, 8), (12, 8)]

@@ -8,22 +8,23 @@
 // g and u are formed again in the kernel that forms dh (three accumulators of one tile) instead of being kept: at the widths
 // of per-atom networks (K <= 1024) the extra 4 M K H operations cost less than writing and reading 2 M H values in 32 bits,
 // and 16-bit copies would add their rounding to every gradient.  What is rounded to 16 bits is what the next product reads:
-// h, dg and du, once each.  Over many rows and columns those roundings average out (the error of a result is sqrt(2) times its
+// h, dg and du, once each (float16: values of h past 65504 become infinite).  Over many rows and columns those roundings average out (the error of a result is sqrt(2) times its
 // own rounding); up to 256 rows, where the products cost next to nothing, they are kept as a 16-bit value and a 16-bit
 // remainder and the next product reads both.
 //
-// Where the contraction axis of a projection (K, or N for dh) is too long for the accumulators of one tile (max_blocks), g, u and
-// dh are formed as float32 matrices by split products and a kernel of its own applies the gate.
+// Where the contraction axis of a projection (K, or N for dh) is too long for the accumulators of one tile (max_blocks: K past
+// 8192 in float16, 65,536 in bfloat16, 2048 in float32), g, u and dh are formed as float32 matrices by split products and a
+// kernel of its own applies the gate.
 //
 // float32 matrices run on the same tensor cores: a value is the exact sum of three bf16 values and a product the six
 // partial products above 2^-24 of it; the intermediate h, dg and du are stored as three planes each, so nothing is lost to
 // 16 bits.  There dh is a product of its own (its accumulators would not fit beside those of g and u).
 //
 // What bounds it (8192 x 1024 -> 4096 -> 1024, bfloat16): the plain products run at 1150 to 1490 TFLOP/s (51 to 58 us of 69
-// GFLOP, 92 to 105 us of 137), tensor-bound up to the last, partly filled round of tiles; both projections with the gate 100 to
-// 113 us (137 GFLOP), the gate's gradient 207 to 215 us (206 GFLOP), whose epilogue is only hidden behind the part of the next
-// tile that forms dh.  Narrow blocks (131,072 x 128 -> 512 -> 128) are bound by the epilogue and by h going through memory:
-// 77 us for h, 33 us for y.  float32 (4096 x 256 -> 1024 -> 256) does six times the products: 264 us forward and backward.
+// GFLOP, 92 to 105 us of 137), tensor-bound up to the last, partly filled round of tiles; both projections with the gate 97 us
+// (137 GFLOP), the gate's gradient 188 us (206 GFLOP), whose epilogue is only hidden behind the part of the next tile that
+// forms dh.  Narrow blocks (131,072 x 128 -> 512 -> 128) are bound by the epilogue and by h going through memory: 72 us for h,
+// 33 us for y.  float32 (4096 x 256 -> 1024 -> 256) does six times the products: 270 us forward and backward.
 #include "dense16.cuh"
 #include "gate.cuh"
 

@@ -21,9 +21,12 @@
 // A and B are symmetric: where the GPU has no tile to spare only those on and below the diagonal are computed, each written
 // twice.
 //
-// What bounds it: 4 x 1024 x 4096 bfloat16 takes 566 us: a step is 32 us for A (540 TFLOP/s of what has to be computed; 128-wide
-// tiles, 144 of them), 18 us for B (one short product and its epilogue) and 57 us for the update (600 TFLOP/s; its epilogue reads
-// and writes X, 270 MB a step in all).  Small problems are bound by latency: 1537 x 515 takes 17 launches of 9 to 14 us.
+// The diagonal of A sums squares, and the tensor core loses up to 1e-7 of such a sum with every instruction: past 65,536 terms (a
+// third of that where the remainders take part) A is formed in parts that are added in fp32 (max_blocks in dense16.cuh).
+//
+// What bounds it: 4 x 1024 x 4096 bfloat16 takes 560 us: a step is 30 us for A (540 TFLOP/s of what has to be computed; 128-wide
+// tiles, 144 of them), 16 us for B (one short product and its epilogue) and 53 us for the update (600 TFLOP/s; its epilogue reads
+// and writes X, 270 MB a step in all).  Small problems are bound by latency: 1537 x 515 takes 187 us, 17 launches of 3 to 12 us.
 #include "dense16.cuh"
 
 namespace nva {

@@ -5,9 +5,9 @@ Weights are ``[in, out]`` like those of :func:`~nvalchemi_toolkit_b200.ops.gemm.
 (``linear.weight.t()``) is read in place as well.  ``gated_feed_forward`` is differentiable;
 ``gated_feed_forward_backward`` is the backward pass on its own, for hand-written steps and for capture into CUDA graphs (it
 involves no autograd graph).  CUDA tensors run ``csrc/feedforward.cu`` on the tensor cores: bfloat16 and float16 with 32-bit
-sums (``h`` and its gradients are rounded to the type once, as the operands of the next product), float32 to 32-bit accuracy
-by exact splits into three bfloat16 parts.  Infinities and NaN give non-finite results (float32: an infinity may come out as
-NaN).  CPU tensors run the same formulas in PyTorch, float64 among them.
+sums (``h`` and its gradients are rounded to the type once, as the operands of the next product; in float16 a value of ``h``
+past 65504 becomes infinite, from 9 rows on), float32 to 32-bit accuracy by exact splits into three bfloat16 parts.  Sums of any
+length keep their accuracy.  Infinities and NaN give non-finite results (float32: an infinity may come out as NaN).  CPU tensors run the same formulas in PyTorch, float64 among them.
 
 Forces are gradients, so training on them differentiates the backward pass once more: the second derivative is the formula of
 the backward pass differentiated by PyTorch, in 32 bits.

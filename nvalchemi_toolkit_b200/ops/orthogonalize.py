@@ -3,8 +3,8 @@
 
 ``newton_schulz(g)`` maps ``G = U S V^T`` to ``U p(S / |G|_F) V^T``, where the odd polynomial ``p`` (``steps`` times
 ``s -> a s + b s^3 + c s^5``) takes every singular value that is not tiny to about 1.  Leading axes are a batch.  CUDA tensors
-run ``csrc/orthogonalize.cu`` on the tensor cores (float16 operands scaled by powers of two, fp32 sums, fp32 iterate); CPU
-tensors run the formula in float32.  The result is a direction, not a sum: it is returned in bfloat16.
+run ``csrc/orthogonalize.cu`` on the tensor cores (float16 operands scaled by powers of two, fp32 sums, the iterate as a float16
+value and a float16 remainder, 22 bits); CPU tensors run the formula in float32.  The result is a direction, not a sum: it is returned in bfloat16.
 """
 from __future__ import annotations
 

@@ -231,6 +231,11 @@ def counts_from_weights(weights: Sequence[float], total: int) -> list[int]:
     return base.tolist()
 
 
+def _padded(items: list, count: int) -> list:
+    """``items`` repeated from its head up to ``count`` elements, as often as that takes."""
+    return items + [items[i % len(items)] for i in range(count - len(items))]
+
+
 class MultiDatasetSampler:
     """Global indices of a :class:`MultiDataset` at per-dataset rates (reference ``data/datapipes/samplers.py:237-420``).
 
@@ -296,9 +301,7 @@ class MultiDatasetSampler:
         per, w = self._per_rank(), self.world_size
         if self.drop_last:
             order = order[: per * w]
-        elif len(order) < per * w:
-            order = order + order[: per * w - len(order)]
-        return iter(order[self.rank:: w])
+        return iter(_padded(order, per * w)[self.rank:: w])
 
 
 class MultiDatasetBatchSampler:
@@ -442,9 +445,7 @@ class FixedCompositionBatchSampler:
         per, w = self._per_rank(), self.world_size
         if self.drop_last:
             batches = batches[: per * w]
-        elif len(batches) < per * w:
-            batches = batches + batches[: per * w - len(batches)]
-        return iter(batches[self.rank:: w])
+        return iter(_padded(batches, per * w)[self.rank:: w])
 
 
 class DataLoader:
@@ -479,7 +480,7 @@ class DataLoader:
             if self.shuffle else list(range(n))
         if self.world_size > 1:
             per = math.ceil(n / self.world_size)
-            order = (order + order[: per * self.world_size - n])[self.rank:: self.world_size]
+            order = _padded(order, per * self.world_size)[self.rank:: self.world_size]
         out = [order[i: i + self.batch_size] for i in range(0, len(order), self.batch_size)]
         if self.drop_last and out and len(out[-1]) < self.batch_size:
             out.pop()

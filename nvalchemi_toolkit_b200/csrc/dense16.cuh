@@ -615,7 +615,7 @@ inline int pick_bn(int64_t tiles256, int64_t tiles128) {
 }
 
 // 64-wide blocks (four instructions each) that may be added to one accumulator.  16 bits: what is lost stays under an eighth of
-// half a step of the result's type, 2^-14 (float16) and 2^-11.  float32: 32 instructions, 7e-7 in sums of both signs and 3.2e-6
+// half a step of the result's type, 2^-14 (float16) and 2^-11.  float32: 32 instructions, 5e-7 in sums of both signs and 3.2e-6
 // at most.
 inline int max_blocks(at::ScalarType t) { return t == at::kFloat ? 8 : t == at::kHalf ? 128 : 1024; }
 
@@ -680,7 +680,8 @@ void run_dense(const Maps& maps, Tiles& t, const typename Epi::Params& ep, cudaS
 
 // out = base (0 if null) + the sum over splits of partial [splits][n], in order.  `base` may be `out`.
 template <typename T>
-__global__ void __launch_bounds__(256) split_sum_kernel(const float* __restrict__ partial, int splits, int64_t stride, int64_t n, const float* base, T* out) {
+__global__ void __launch_bounds__(256) split_sum_kernel(const float* __restrict__ partial, int splits, int64_t stride, int64_t n,
+                                                        const float* base, T* out) {
   chain_wait();
   const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
   if (i >= n) return;

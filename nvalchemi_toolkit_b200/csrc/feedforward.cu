@@ -8,9 +8,9 @@
 // g and u are formed again in the kernel that forms dh (three accumulators of one tile) instead of being kept: at the widths
 // of per-atom networks (K <= 1024) the extra 4 M K H operations cost less than writing and reading 2 M H values in 32 bits,
 // and 16-bit copies would add their rounding to every gradient.  What is rounded to 16 bits is what the next product reads:
-// h, dg and du, once each (float16: values of h past 65504 become infinite).  Over many rows and columns those roundings average out (the error of a result is sqrt(2) times its
-// own rounding); up to 256 rows, where the products cost next to nothing, they are kept as a 16-bit value and a 16-bit
-// remainder and the next product reads both.
+// h, dg and du, once each (float16: values of h past 65504 become infinite).  Over many rows and columns those roundings average
+// out (the error of a result is sqrt(2) times its own rounding); up to 256 rows, where the products cost next to nothing, they
+// are kept as a 16-bit value and a 16-bit remainder and the next product reads both.
 //
 // Where the contraction axis of a projection (K, or N for dh) is too long for the accumulators of one tile (max_blocks: K past
 // 8192 in float16, 65,536 in bfloat16, 2048 in float32), g, u and dh are formed as float32 matrices by split products and a
